@@ -20,6 +20,7 @@
 #include "sm_count.h"
 
 void register_conv(pybind11::module& m);
+void register_lm(pybind11::module& m);
 
 namespace {
 
@@ -1249,4 +1250,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("relaxed_pull", &relaxed_pull);
   m.attr("MAX_COMM_BLOCKS") = adb200::kMaxCommBlocks;
   register_conv(m);
+  register_lm(m);
 }

@@ -1,0 +1,392 @@
+// Python bindings of a recurrent language model's operators: argument checks, outputs, launches on the current stream of the tensors' GPU.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <cuda_runtime.h>
+#include <torch/extension.h>
+
+#include <memory>
+#include <string>
+#include <vector>
+
+#include "adamw_list.h"
+#include "gemm_8bit.h"
+#include "recurrence.h"
+#include "rms_norm.h"
+
+namespace {
+
+using at::Tensor;
+using c10::optional;
+
+// A tensor's shape and type for a message. Put together here: the library's stream operator for shapes crashed in this extension.
+std::string shown(const Tensor& t) {
+  std::string r = "[";
+  for (int64_t d = 0; d < t.dim(); ++d) r += (d ? ", " : "") + std::to_string(t.size(d));
+  return r + "] " + c10::toString(t.scalar_type());
+}
+
+void launched(cudaError_t e, const char* what) { TORCH_CHECK(e == cudaSuccess, what, ": ", cudaGetErrorString(e)); }
+
+cudaStream_t stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+
+bool same_gpu(const Tensor& a, const Tensor& b) { return b.is_cuda() && b.device() == a.device(); }
+void check_gpu(const Tensor& a, const optional<Tensor>& b, const char* name) {
+  TORCH_CHECK(!b.has_value() || same_gpu(a, *b), name, ": tensors on one GPU needed");
+}
+
+// Whether a stream's type is bf16; fp32 is the other one.
+bool is_bf16(const Tensor& t, const char* name) {
+  TORCH_CHECK(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat, name, ": bf16 or fp32 needed, got ", shown(t));
+  return t.scalar_type() == at::kBFloat16;
+}
+
+// [..., width] as [rows, width] with unit stride along the width: a view where the strides allow it.
+Tensor as_rows(const Tensor& t) {
+  Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
+  return r.stride(1) == 1 || r.size(1) == 1 ? r : r.contiguous();
+}
+// From one row to the next; a single row's stride means nothing.
+int64_t row_stride(const Tensor& rows) { return rows.size(0) > 1 ? rows.stride(0) : rows.size(1); }
+
+// ---------------------------------------------------------------------------------------------- norm
+int64_t check_width(const Tensor& x, const char* name) {
+  TORCH_CHECK(x.is_cuda(), name, ": a tensor on a GPU needed");
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, name, ": rows of at least one element needed");
+  TORCH_CHECK(x.size(-1) < (1LL << 30), name, ": rows too wide");
+  return x.size(-1);
+}
+void check_like(const Tensor& x, const optional<Tensor>& other, const char* name, const char* what) {
+  if (!other.has_value()) return;
+  TORCH_CHECK(same_gpu(x, *other), name, ": ", what, " must be on the input's GPU");
+  TORCH_CHECK(other->sizes() == x.sizes() && other->scalar_type() == x.scalar_type(), name, ": ", what, " must have the input's shape and type, got ",
+              shown(*other), " for ", shown(x));
+}
+Tensor check_weight(const Tensor& x, const Tensor& weight, const char* name) {
+  TORCH_CHECK(same_gpu(x, weight), name, ": the weight must be on the input's GPU");
+  TORCH_CHECK(weight.dim() == 1 && weight.size(0) == x.size(-1), name, ": a weight for each column needed, got ", shown(weight), " for ", shown(x));
+  TORCH_CHECK(weight.scalar_type() == at::kFloat || weight.scalar_type() == x.scalar_type(), name, ": the weight must be fp32 or of the input's type, got ", shown(weight));
+  return weight.contiguous();
+}
+
+struct NormInputs {                        // what the addresses in `rows` belong to
+  Tensor x, res, weight, sum;
+  adb200::NormRows rows{};
+};
+NormInputs norm_inputs(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& residual, double eps, const char* name) {
+  const int64_t width = check_width(x, name);
+  NormInputs in;
+  in.rows.bf16 = is_bf16(x, name);
+  check_like(x, residual, name, "the residual");
+  if (weight.has_value()) {
+    in.weight = check_weight(x, *weight, name);
+    in.rows.weight = in.weight.data_ptr();
+    in.rows.weight_bf16 = in.weight.scalar_type() == at::kBFloat16;
+  }
+  in.x = as_rows(x);
+  in.rows.x = in.x.data_ptr();
+  in.rows.x_ld = row_stride(in.x);
+  if (residual.has_value()) {
+    in.res = as_rows(*residual);
+    in.rows.res = in.res.data_ptr();
+    in.rows.res_ld = row_stride(in.res);
+    in.sum = at::empty(x.sizes(), x.options());
+    in.rows.sum = in.sum.data_ptr();
+  }
+  in.rows.rows = in.x.size(0);
+  in.rows.width = (int)width;
+  in.rows.eps = (float)eps;
+  return in;
+}
+
+// -> (y, x + residual)
+std::tuple<Tensor, optional<Tensor>> rms_norm_fwd(const Tensor& x, const Tensor& weight, const optional<Tensor>& residual, double eps) {
+  TORCH_CHECK(x.is_cuda(), "rms_norm: a tensor on a GPU needed");
+  const c10::cuda::CUDAGuard guard(x.device());
+  NormInputs in = norm_inputs(x, weight, residual, eps, "rms_norm");
+  Tensor y = at::empty(x.sizes(), x.options());
+  launched(adb200::rms_norm_fwd(in.rows, y.data_ptr(), stream_of(x)), "rms_norm");
+  return {y, residual.has_value() ? optional<Tensor>(in.sum) : c10::nullopt};
+}
+
+// -> (gradient of the input and of the residual, gradient of the weight)
+std::tuple<Tensor, Tensor> rms_norm_bwd(const Tensor& dy, const optional<Tensor>& ds, const Tensor& s, const Tensor& weight, double eps) {
+  const char* name = "rms_norm";
+  TORCH_CHECK(s.is_cuda(), "rms_norm: a tensor on a GPU needed");
+  const c10::cuda::CUDAGuard guard(s.device());
+  const int64_t width = check_width(s, name);
+  check_like(s, dy, name, "the gradient");
+  check_like(s, ds, name, "the sum's gradient");
+  adb200::NormGrad g{};
+  g.bf16 = is_bf16(s, name);
+  const Tensor w = check_weight(s, weight, name), rows = as_rows(s), dyr = as_rows(dy);
+  Tensor dsr;
+  g.dy = dyr.data_ptr(); g.dy_ld = row_stride(dyr);
+  if (ds.has_value()) {
+    dsr = as_rows(*ds);
+    g.ds = dsr.data_ptr(); g.ds_ld = row_stride(dsr);
+  }
+  g.s = rows.data_ptr(); g.s_ld = row_stride(rows);
+  g.weight = w.data_ptr(); g.weight_bf16 = w.scalar_type() == at::kBFloat16;
+  g.rows = rows.size(0); g.width = (int)width; g.eps = (float)eps;
+  Tensor dx = at::empty(s.sizes(), s.options()), dw = at::empty(w.sizes(), w.options());
+  Tensor part = at::empty({(int64_t)adb200::rms_norm_bwd_parts(g.rows, g.width) * width}, s.options().dtype(at::kFloat));
+  g.dx = dx.data_ptr(); g.dw = dw.data_ptr(); g.part = part.data_ptr<float>();
+  launched(adb200::rms_norm_bwd(g, stream_of(s)), name);
+  return {dx, dw};
+}
+
+// Codes of [..., width] whose rows start on 16-byte boundaries.
+Tensor empty_codes(const Tensor& x) {
+  std::vector<int64_t> shape = x.sizes().vec();
+  const int64_t width = shape.back();
+  shape.back() = (width + 15) / 16 * 16;
+  Tensor t = at::empty(shape, x.options().dtype(at::kFloat8_e4m3fn));
+  return shape.back() == width ? t : t.narrow(-1, 0, width);
+}
+std::tuple<Tensor, Tensor, optional<Tensor>> rows_8bit(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& residual, double eps,
+                                                       const char* name) {
+  TORCH_CHECK(x.is_cuda(), name, ": a tensor on a GPU needed");
+  const c10::cuda::CUDAGuard guard(x.device());
+  NormInputs in = norm_inputs(x, weight, residual, eps, name);
+  Tensor codes = empty_codes(x), scales = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+  launched(adb200::rms_norm_8bit(in.rows, codes.data_ptr(), (in.rows.width + 15) / 16 * 16, scales.data_ptr<float>(), stream_of(x)), name);
+  return {codes, scales, residual.has_value() ? optional<Tensor>(in.sum) : c10::nullopt};
+}
+// -> (codes, scales, x + residual)
+std::tuple<Tensor, Tensor, optional<Tensor>> rms_norm_8bit(const Tensor& x, const Tensor& weight, const optional<Tensor>& residual, double eps) {
+  return rows_8bit(x, weight, residual, eps, "rms_norm_8bit");
+}
+std::tuple<Tensor, Tensor> quantize_rows(const Tensor& x) {
+  auto r = rows_8bit(x, c10::nullopt, c10::nullopt, 0.0, "quantize_rows");
+  return {std::get<0>(r), std::get<1>(r)};
+}
+
+// ---------------------------------------------------------------------------------------------- product
+// Rows of codes as the kernels read them: on 16-byte boundaries.
+Tensor aligned_codes(const Tensor& t, const char* what) {
+  TORCH_CHECK(t.scalar_type() == at::kFloat8_e4m3fn && t.dim() >= 1, "linear_8bit: ", what, " must be float8_e4m3fn, got ", shown(t));
+  TORCH_CHECK(t.size(-1) > 0 && t.size(-1) < (1LL << 30), "linear_8bit: ", what, " must have between 1 and 2^30 columns, got ", shown(t));
+  Tensor r = as_rows(t);
+  if (reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 == 0 && row_stride(r) % 16 == 0 && row_stride(r) >= r.size(1)) return r;
+  if (r.size(0) <= 1 && reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 == 0) return r;
+  return empty_codes(r).copy_(r);
+}
+int64_t code_stride(const Tensor& r) { return r.size(0) > 1 ? r.stride(0) : (r.size(1) + 15) / 16 * 16; }
+
+Tensor gemm_8bit(const Tensor& codes, const Tensor& scales, const Tensor& weight_codes, const Tensor& weight_scales, const optional<Tensor>& bias, Tensor error) {
+  const char* name = "linear_8bit";
+  TORCH_CHECK(codes.is_cuda(), "linear_8bit: tensors on a GPU needed");
+  check_gpu(codes, scales, name); check_gpu(codes, weight_codes, name); check_gpu(codes, weight_scales, name); check_gpu(codes, bias, name);
+  check_gpu(codes, error, name);
+  const c10::cuda::CUDAGuard guard(codes.device());
+  TORCH_CHECK(weight_codes.dim() == 2 && codes.size(-1) == weight_codes.size(1), "linear_8bit: rows of ", shown(codes), " and weights of ", shown(weight_codes),
+              " do not match");
+  const Tensor x = aligned_codes(codes, "the rows"), w = aligned_codes(weight_codes, "the weight");
+  const int64_t M = x.size(0), N = w.size(0);
+  TORCH_CHECK(M < (1LL << 31) && N < (1LL << 31), "linear_8bit: too many rows");
+  TORCH_CHECK(scales.scalar_type() == at::kFloat && scales.numel() == M && weight_scales.scalar_type() == at::kFloat && weight_scales.numel() == N,
+              "linear_8bit: an fp32 scale for each row needed");
+  TORCH_CHECK(!bias.has_value() || (bias->scalar_type() == at::kFloat && bias->numel() == N), "linear_8bit: an fp32 bias for each output needed");
+  TORCH_CHECK(error.scalar_type() == at::kInt && error.numel() >= 1, "linear_8bit: an int32 word needed");
+  const Tensor sx = scales.contiguous(), sw = weight_scales.contiguous(), b = bias.has_value() ? bias->contiguous() : Tensor();
+  std::vector<int64_t> shape = codes.sizes().vec();
+  shape.back() = N;
+  Tensor y = at::empty(shape, codes.options().dtype(at::kBFloat16));
+  adb200::Gemm8Args a{};
+  a.codes = static_cast<const uint8_t*>(x.data_ptr()); a.codes_ld = code_stride(x);
+  a.scales = sx.data_ptr<float>();
+  a.weight_codes = static_cast<const uint8_t*>(w.data_ptr()); a.weight_ld = code_stride(w);
+  a.weight_scales = sw.data_ptr<float>();
+  a.bias = b.defined() ? b.data_ptr<float>() : nullptr;
+  a.y = y.data_ptr();
+  a.M = (int)M; a.N = (int)N; a.K = (int)x.size(1);
+  a.error = error.data_ptr<int>();
+  launched(adb200::gemm_8bit(a, stream_of(codes)), name);
+  return y;
+}
+
+// ---------------------------------------------------------------------------------------------- recurrence
+struct ScanInputs {                        // what the addresses in `a` belong to
+  Tensor x, forget, input, state, reset;
+  adb200::ScanArgs a{};
+};
+adb200::ScanView scan_view(const Tensor& t, Tensor& held) {
+  held = t.stride(2) == 1 || t.size(2) == 1 ? t : t.contiguous();
+  return {held.data_ptr(), held.stride(0), held.stride(1)};
+}
+ScanInputs scan_inputs(const Tensor& x, const Tensor& forget, const optional<Tensor>& input, const optional<Tensor>& state, const optional<Tensor>& reset,
+                       double forget_bias) {
+  const char* name = "gated_recurrence";
+  TORCH_CHECK(x.dim() == 3, "gated_recurrence: [batch, steps, channels] needed, got ", shown(x));
+  ScanInputs in;
+  in.a.bf16 = is_bf16(x, name);
+  check_like(x, forget, name, "the forget gate");
+  check_like(x, input, name, "the input gate");
+  const int64_t B = x.size(0), T = x.size(1), C = x.size(2);
+  TORCH_CHECK(T < (1LL << 31) && B * ((C + 31) / 32) < (1LL << 31) / 64, "gated_recurrence: too large");
+  in.a.x = scan_view(x, in.x);
+  in.a.forget = scan_view(forget, in.forget);
+  if (input.has_value()) in.a.input = scan_view(*input, in.input);
+  if (state.has_value()) {
+    TORCH_CHECK(same_gpu(x, *state) && state->scalar_type() == at::kFloat && state->dim() == 2 && state->size(0) == B && state->size(1) == C,
+                "gated_recurrence: an fp32 state [batch, channels] on the input's GPU needed, got ", shown(*state));
+    in.state = state->contiguous();
+    in.a.state = in.state.data_ptr<float>();
+  }
+  if (reset.has_value()) {
+    TORCH_CHECK(same_gpu(x, *reset) && reset->scalar_type() == at::kBool && reset->dim() == 2 && reset->size(0) == B && reset->size(1) == T,
+                "gated_recurrence: a bool reset [batch, steps] on the input's GPU needed, got ", shown(*reset));
+    in.reset = *reset;
+    in.a.reset = static_cast<const uint8_t*>(reset->data_ptr());
+    in.a.reset_batch = reset->stride(0);
+    in.a.reset_step = reset->stride(1);
+  }
+  in.a.batch = (int)B; in.a.steps = (int)T; in.a.channels = (int)C;
+  in.a.forget_bias = (float)forget_bias;
+  return in;
+}
+
+// -> (outputs, last state, states kept for the backward pass)
+std::tuple<Tensor, Tensor, optional<Tensor>> gated_scan_fwd(const Tensor& x, const Tensor& forget, const optional<Tensor>& input, const optional<Tensor>& state,
+                                                            const optional<Tensor>& reset, double forget_bias, bool keep) {
+  TORCH_CHECK(x.is_cuda(), "gated_recurrence: tensors on a GPU needed");
+  const c10::cuda::CUDAGuard guard(x.device());
+  ScanInputs in = scan_inputs(x, forget, input, state, reset, forget_bias);
+  const auto f32 = x.options().dtype(at::kFloat);
+  Tensor y = at::empty(x.sizes(), x.options()), last = at::empty({x.size(0), x.size(2)}, f32), kept;
+  if (keep) kept = at::empty({x.size(0), (x.size(1) + adb200::kScanTile - 1) / adb200::kScanTile, x.size(2)}, f32);
+  launched(adb200::gated_scan_fwd(in.a, y.data_ptr(), last.data_ptr<float>(), keep ? kept.data_ptr<float>() : nullptr, stream_of(x)), "gated_recurrence");
+  return {y, last, keep ? optional<Tensor>(kept) : c10::nullopt};
+}
+
+// -> gradients of (x, forget, input, state)
+std::tuple<Tensor, Tensor, optional<Tensor>, Tensor> gated_scan_bwd(const optional<Tensor>& dy, const optional<Tensor>& dlast, const Tensor& x, const Tensor& forget,
+                                                                    const optional<Tensor>& input, const optional<Tensor>& state, const optional<Tensor>& reset,
+                                                                    const Tensor& kept, double forget_bias) {
+  TORCH_CHECK(x.is_cuda(), "gated_recurrence: tensors on a GPU needed");
+  const c10::cuda::CUDAGuard guard(x.device());
+  ScanInputs in = scan_inputs(x, forget, input, state, reset, forget_bias);
+  check_like(x, dy, "gated_recurrence", "the gradient");
+  const int64_t B = x.size(0), C = x.size(2);
+  TORCH_CHECK(same_gpu(x, kept) && kept.scalar_type() == at::kFloat && kept.is_contiguous() &&
+                  kept.numel() == B * C * ((x.size(1) + adb200::kScanTile - 1) / adb200::kScanTile), "gated_recurrence: the forward pass's states needed");
+  adb200::ScanGrads g{};
+  Tensor dy_held, dlast_held;
+  if (dy.has_value()) g.dy = scan_view(*dy, dy_held);
+  if (dlast.has_value()) {
+    TORCH_CHECK(same_gpu(x, *dlast) && dlast->scalar_type() == at::kFloat && dlast->numel() == B * C, "gated_recurrence: an fp32 gradient of the last state needed");
+    dlast_held = dlast->contiguous();
+    g.dlast = dlast_held.data_ptr<float>();
+  }
+  Tensor dx = at::empty(x.sizes(), x.options()), dforget = at::empty(x.sizes(), x.options()), dstate = at::empty({B, C}, kept.options()), dinput;
+  if (input.has_value()) dinput = at::empty(x.sizes(), x.options());
+  g.kept = kept.data_ptr<float>();
+  g.dx = dx.data_ptr(); g.dforget = dforget.data_ptr(); g.dinput = input.has_value() ? dinput.data_ptr() : nullptr; g.dstate = dstate.data_ptr<float>();
+  launched(adb200::gated_scan_bwd(in.a, g, stream_of(x)), "gated_recurrence");
+  return {dx, dforget, input.has_value() ? optional<Tensor>(dinput) : c10::nullopt, dstate};
+}
+
+// ---------------------------------------------------------------------------------------------- optimizer
+// The parameters of a group and where their moments lie. Addresses are read at every step: a parameter's storage may change.
+struct AdamwList {
+  std::vector<Tensor> params;
+  std::vector<int64_t> places;             // first element of each parameter's moments
+  Tensor m, r, m_scale, r_scale, step;
+  uint64_t seed = 0;
+};
+
+std::shared_ptr<AdamwList> adamw_list(std::vector<Tensor> params, std::vector<int64_t> places, Tensor m, Tensor r, const optional<Tensor>& m_scale,
+                                      const optional<Tensor>& r_scale, Tensor step, int64_t seed) {
+  TORCH_CHECK(!params.empty() && params.size() == places.size(), "adamw: a place for each parameter needed");
+  const bool bits8 = m_scale.has_value();
+  const auto type = bits8 ? at::kFloat8_e4m3fn : at::kFloat;
+  for (const Tensor* t : {&m, &r})
+    TORCH_CHECK(same_gpu(params[0], *t) && t->scalar_type() == type && t->is_contiguous() && t->numel() % adb200::kAdamwBlock == 0, "adamw: bad moments");
+  TORCH_CHECK(r.numel() == m.numel() && r_scale.has_value() == bits8, "adamw: bad moments");
+  if (bits8)
+    for (const Tensor* t : {&*m_scale, &*r_scale})
+      TORCH_CHECK(same_gpu(params[0], *t) && t->scalar_type() == at::kFloat && t->is_contiguous() && t->numel() == m.numel() / adb200::kAdamwBlock, "adamw: bad scales");
+  TORCH_CHECK(same_gpu(params[0], step) && step.scalar_type() == at::kLong && step.is_contiguous() && step.numel() == 2, "adamw: a counter of two words needed");
+  for (size_t i = 0; i < params.size(); ++i) {
+    TORCH_CHECK(same_gpu(params[0], params[i]), "adamw: parameters on one GPU needed");
+    is_bf16(params[i], "adamw");
+    TORCH_CHECK(places[i] >= 0 && places[i] % adb200::kAdamwBlock == 0 && places[i] + params[i].numel() <= m.numel(), "adamw: a parameter's moments lie outside");
+  }
+  auto list = std::make_shared<AdamwList>();
+  list->params = std::move(params);
+  list->places = std::move(places);
+  list->m = m; list->r = r;
+  if (bits8) { list->m_scale = *m_scale; list->r_scale = *r_scale; }
+  list->step = step;
+  list->seed = (uint64_t)seed;
+  return list;
+}
+
+// One step over the parameters that have a gradient. Returns how many kernels it launched.
+int64_t adamw_list_step(const std::shared_ptr<AdamwList>& l, double lr, const optional<Tensor>& lr_at, double b1, double b2, double eps, double wd) {
+  const Tensor& first = l->params[0];
+  const c10::cuda::CUDAGuard guard(first.device());
+  const cudaStream_t st = stream_of(first);
+  if (lr_at.has_value()) TORCH_CHECK(same_gpu(first, *lr_at) && lr_at->scalar_type() == at::kFloat && lr_at->numel() == 1, "adamw: an fp32 learning rate on the GPU needed");
+  struct Batch { bool p16, g16; std::unique_ptr<adb200::AdamwTable> table; };
+  std::vector<Batch> batches;
+  std::vector<Tensor> held;                                  // gradients and parameters that had to be laid out
+  std::vector<std::pair<Tensor, Tensor>> back;               // parameters to copy into, from their laid-out copies
+  for (size_t i = 0; i < l->params.size(); ++i) {
+    Tensor p = l->params[i], g = p.grad();
+    if (!g.defined() || p.numel() == 0) continue;
+    TORCH_CHECK(!g.is_sparse(), "adamw: sparse gradients are not supported");
+    TORCH_CHECK(same_gpu(first, p) && same_gpu(first, g) && g.numel() == p.numel() && g.sizes() == p.sizes(), "adamw: a gradient does not match its parameter");
+    const bool p16 = is_bf16(p, "adamw"), g16 = is_bf16(g, "adamw");
+    if (!g.is_contiguous()) held.push_back(g = g.contiguous());
+    if (!p.is_contiguous()) {
+      Tensor c = p.detach().contiguous();
+      back.emplace_back(p, c);
+      p = c;
+    }
+    const int64_t chunks = (p.numel() + adb200::kAdamwChunk - 1) / adb200::kAdamwChunk;
+    TORCH_CHECK(chunks < (1LL << 30), "adamw: a parameter is too large");
+    Batch* b = nullptr;
+    for (Batch& c : batches)
+      if (c.p16 == p16 && c.g16 == g16 && c.table->count < adb200::kAdamwMost && c.table->first[c.table->count] + chunks < (1LL << 30)) b = &c;
+    if (b == nullptr) {
+      batches.push_back({p16, g16, std::make_unique<adb200::AdamwTable>()});
+      b = &batches.back();
+      b->table->count = 0;
+      b->table->first[0] = 0;
+    }
+    adb200::AdamwTable& t = *b->table;
+    t.t[t.count] = {p.data_ptr(), g.data_ptr(), p.numel(), l->places[i]};
+    t.first[t.count + 1] = t.first[t.count] + (int)chunks;
+    ++t.count;
+  }
+  const bool bits8 = l->m_scale.defined();
+  const adb200::AdamwMoments mo{l->m.data_ptr(), l->r.data_ptr(), bits8 ? l->m_scale.data_ptr<float>() : nullptr, bits8 ? l->r_scale.data_ptr<float>() : nullptr};
+  adb200::AdamwRule rule{b1, b2, eps, wd, lr_at.has_value() ? lr_at->data_ptr<float>() : nullptr, lr, l->seed,
+                         reinterpret_cast<long long*>(l->step.data_ptr<int64_t>()), 0};
+  for (size_t k = 0; k < batches.size(); ++k) {
+    rule.advance = k + 1 == batches.size();
+    launched(adb200::adamw_list_step(*batches[k].table, batches[k].p16, batches[k].g16, mo, rule, st), "adamw");
+  }
+  for (auto& b : back) {
+    at::NoGradGuard no_grad;
+    b.first.detach().copy_(b.second);
+  }
+  return (int64_t)batches.size();
+}
+
+}  // namespace
+
+void register_lm(pybind11::module& m) {
+  m.def("rms_norm_fwd", &rms_norm_fwd);
+  m.def("rms_norm_bwd", &rms_norm_bwd);
+  m.def("rms_norm_8bit", &rms_norm_8bit);
+  m.def("quantize_rows", &quantize_rows);
+  m.def("gemm_8bit", &gemm_8bit);
+  m.def("gated_scan_fwd", &gated_scan_fwd);
+  m.def("gated_scan_bwd", &gated_scan_bwd);
+  pybind11::class_<AdamwList, std::shared_ptr<AdamwList>>(m, "_AdamwList");
+  m.def("adamw_list", &adamw_list);
+  m.def("adamw_list_step", &adamw_list_step);
+  m.attr("ADAMW_BLOCK") = adb200::kAdamwBlock;
+}

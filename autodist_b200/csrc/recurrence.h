@@ -1,0 +1,33 @@
+// Host-side interface of the gated linear recurrence (see recurrence.cu).
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace adb200 {
+
+constexpr int kScanTile = 128;             // steps between the states that the forward pass keeps for the backward pass
+
+// [batch, steps, channels] views with unit stride along channels; strides in elements.
+struct ScanView { const void* p; long long batch, step; };
+struct ScanArgs {
+  ScanView x, forget, input;               // input.p == nullptr: the input is weighted by 1 - forget
+  const float* state;                      // [batch, channels]; nullptr: zeros
+  const uint8_t* reset; long long reset_batch, reset_step;      // [batch, steps]; nullptr: none
+  int batch, steps, channels;
+  float forget_bias;
+  bool bf16;                               // else fp32
+};
+// y: [batch, steps, channels], last: [batch, channels]; kept (nullptr: not wanted): [batch, ceil(steps / kScanTile), channels], the states in front
+// of each tile
+cudaError_t gated_scan_fwd(const ScanArgs& a, void* y, float* last, float* kept, cudaStream_t st);
+
+struct ScanGrads {
+  ScanView dy;                             // p == nullptr: zeros
+  const float* dlast;                      // nullptr: zeros
+  const float* kept;
+  void *dx, *dforget, *dinput;             // [batch, steps, channels]; dinput only with an input gate
+  float* dstate;                           // [batch, channels]
+};
+cudaError_t gated_scan_bwd(const ScanArgs& a, const ScanGrads& g, cudaStream_t st);
+
+}  // namespace adb200

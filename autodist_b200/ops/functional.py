@@ -12,6 +12,7 @@ import torch
 import torch.nn.functional as F
 
 from autodist_b200 import ops
+from autodist_b200.ops.lm import gated_recurrence, linear_8bit, quantize_rows, rms_norm, rms_norm_8bit  # noqa: F401 (the public names)
 
 _err = {}
 

@@ -1,0 +1,212 @@
+"""Operators of a gated recurrent language model: root-mean-square norm (with the residual's addition; with an output in 8 bits), a gated
+linear recurrence over time, and the product of 8-bit rows.
+
+CUDA tensors run on the hand-written kernels, CPU tensors on the plain PyTorch expressions below, which are also what second
+derivatives, forward-mode derivatives and ``torch.func`` transforms go through.
+"""
+import torch
+import torch.nn.functional as F
+
+from autodist_b200 import ops
+
+#: Largest e4m3 value: a row in 8 bits is scaled so that its largest element has this size.
+E4M3_MAX = 448.0
+
+_STREAM_TYPES = (torch.bfloat16, torch.float32)
+
+
+def _kernels(x):
+    """Whether the kernels compute this: tensors on a GPU, and no transform but reverse-mode differentiation going on."""
+    return x.is_cuda and not torch._C._are_functorch_transforms_active() and torch.autograd.forward_ad._current_level < 0
+
+
+def _wants_gradient(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _differentiated_again(plain, inputs, needed, grads_of_outputs):
+    """Gradients of ``plain(*inputs)`` that can be differentiated themselves (``create_graph``), ``None`` where none is needed."""
+    wanted = [t for t, w in zip(inputs, needed) if w]
+    outs, grads = zip(*((o, g) for o, g in zip(plain(*inputs), grads_of_outputs) if g is not None))
+    found = iter(torch.autograd.grad(outs, wanted, grads, create_graph=True, allow_unused=True))
+    return [next(found) if w else None for w in needed]
+
+
+# ---------------------------------------------------------------------------------------------------------------- norm
+def _check_norm(name, x, weight, residual):
+    if x.dtype not in _STREAM_TYPES:
+        raise TypeError(f"{name}: bf16 or fp32 needed, got {x.dtype}")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"{name}: rows of at least one element needed, got {tuple(x.shape)}")
+    if weight.shape != x.shape[-1:]:
+        raise ValueError(f"{name}: a weight for each column needed, got {tuple(weight.shape)} for {tuple(x.shape)}")
+    if weight.dtype not in (torch.float32, x.dtype):
+        raise TypeError(f"{name}: the weight must be fp32 or of the input's type, got {weight.dtype}")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError(f"{name}: the residual must have the input's shape and type, got {tuple(residual.shape)} {residual.dtype}")
+
+
+def _norm_plain(x, weight, residual, eps):
+    s = x if residual is None else x + residual
+    f = s.float()
+    y = f * torch.rsqrt(f.square().mean(-1, keepdim=True) + eps) * weight.float()
+    return y, s
+
+
+class _RMSNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        y, s = ops.ext(required=True).rms_norm_fwd(x, weight, residual, eps)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x if residual is None else s, weight)
+        ctx.eps = eps
+        return (y, s) if residual is not None else y
+
+    @staticmethod
+    def backward(ctx, dy, ds=None):
+        s, weight = ctx.saved_tensors
+        need_x, need_w, need_r, _ = ctx.needs_input_grad
+        if dy is None:
+            return ds if need_x else None, None, ds if need_r else None, None
+        if torch.is_grad_enabled():
+            # the sum is the only place where x and the residual meet: both get its gradient
+            dx, dw = _differentiated_again(lambda t, w: (_norm_plain(t, w, None, ctx.eps)[0].to(t.dtype), t), (s, weight),
+                                           (need_x or need_r, need_w), (dy, ds))
+        else:
+            dx, dw = ops.ext(required=True).rms_norm_bwd(dy, ds, s, weight, ctx.eps)
+        return dx if need_x else None, dw if need_w else None, dx if need_r else None, None
+
+
+def rms_norm(x, weight, residual=None, eps=1e-6):
+    """``s * rsqrt(mean(s^2) + eps) * weight`` over the last dimension, with ``s = x``, or ``s = x + residual`` rounded to their type; then
+    ``(norm, s)`` is returned. bf16 or fp32; the weight in fp32 or in the input's type. Sums are fp32."""
+    _check_norm("rms_norm", x, weight, residual)
+    if not _kernels(x):
+        y, s = _norm_plain(x, weight, residual, eps)
+        return y.to(x.dtype) if residual is None else (y.to(x.dtype), s)
+    if _wants_gradient(x, weight, residual):
+        return _RMSNormFn.apply(x, weight, residual, eps)
+    y, s = ops.ext(required=True).rms_norm_fwd(x, weight, residual, eps)
+    return y if residual is None else (y, s)
+
+
+def _no_gradient(name, *tensors):
+    if _wants_gradient(*tensors):
+        raise RuntimeError(f"{name}: rows in 8 bits carry no gradient; call it under torch.no_grad()")
+
+
+def _codes_plain(y):
+    scale = y.abs().amax(-1) / E4M3_MAX
+    held = torch.where(scale[..., None] == 0, torch.zeros_like(y), y / scale[..., None])
+    return held.clamp(-E4M3_MAX, E4M3_MAX).to(torch.float8_e4m3fn), scale
+
+
+def rms_norm_8bit(x, weight, residual=None, eps=1e-6):
+    """``rms_norm`` with its output in 8 bits: ``(codes, scales)``, or ``(codes, scales, s)`` with a residual. ``codes`` (``float8_e4m3fn``)
+    times its row's fp32 scale is the norm's output, the row's largest element being 448 scales; rows of zeros have the scale 0. Rows of
+    ``codes`` start on 16-byte boundaries, as ``linear_8bit`` reads them. Not differentiable."""
+    _check_norm("rms_norm_8bit", x, weight, residual)
+    _no_gradient("rms_norm_8bit", x, weight, residual)
+    if not _kernels(x):
+        y, s = _norm_plain(x, weight, residual, eps)
+        return _codes_plain(y) if residual is None else _codes_plain(y) + (s,)
+    codes, scales, s = ops.ext(required=True).rms_norm_8bit(x, weight, residual, eps)
+    return (codes, scales) if residual is None else (codes, scales, s)
+
+
+def quantize_rows(x):
+    """``(codes, scales)`` of the rows of ``x`` (bf16 or fp32, last dimension) as ``rms_norm_8bit`` returns them: for weights, once, and for
+    activations that no norm produces. Not differentiable: a trained weight is passed detached."""
+    if x.dtype not in _STREAM_TYPES:
+        raise TypeError(f"quantize_rows: bf16 or fp32 needed, got {x.dtype}")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"quantize_rows: rows of at least one element needed, got {tuple(x.shape)}")
+    _no_gradient("quantize_rows", x)
+    return ops.ext(required=True).quantize_rows(x) if _kernels(x) else _codes_plain(x.float())
+
+
+# ---------------------------------------------------------------------------------------------------------------- product in 8 bits
+def linear_8bit(codes, scales, weight_codes, weight_scales, bias=None):
+    """``(codes * scales) @ (weight_codes * weight_scales).T + bias`` in bf16 for rows ``[..., K]`` and a weight ``[N, K]`` of
+    ``float8_e4m3fn`` with an fp32 scale each (``rms_norm_8bit``, ``quantize_rows``). Products are exact, sums fp32. Not differentiable."""
+    if codes.dtype != torch.float8_e4m3fn or weight_codes.dtype != torch.float8_e4m3fn:
+        raise TypeError(f"linear_8bit: float8_e4m3fn rows and weight needed, got {codes.dtype} and {weight_codes.dtype}")
+    if codes.dim() < 1 or weight_codes.dim() != 2 or codes.shape[-1] != weight_codes.shape[1] or codes.shape[-1] < 1:
+        raise ValueError(f"linear_8bit: rows of {tuple(codes.shape)} and a weight of {tuple(weight_codes.shape)} do not match")
+    if scales.dtype != torch.float32 or scales.shape != codes.shape[:-1] or weight_scales.dtype != torch.float32 or \
+            weight_scales.shape != weight_codes.shape[:1]:
+        raise ValueError("linear_8bit: an fp32 scale for each row of both sides needed")
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != weight_scales.shape):
+        raise ValueError("linear_8bit: an fp32 bias for each output needed")
+    _no_gradient("linear_8bit", scales, weight_scales, bias)
+    if codes.is_cuda:
+        from autodist_b200.ops.functional import _error_flag
+        return ops.ext(required=True).gemm_8bit(codes, scales, weight_codes, weight_scales, bias, _error_flag(codes.device))
+    y = F.linear(codes.float(), weight_codes.float()) * scales[..., None] * weight_scales
+    return (y if bias is None else y + bias).to(torch.bfloat16)
+
+
+# ---------------------------------------------------------------------------------------------------------------- recurrence
+def _scan_plain(x, forget, input_gate, state, reset, forget_bias):
+    f = torch.sigmoid(forget.float() + forget_bias)
+    u = torch.sigmoid(-(forget.float() + forget_bias)) if input_gate is None else torch.sigmoid(input_gate.float())
+    v = u * x.float()
+    h = x.new_zeros(x.shape[0], x.shape[2], dtype=torch.float32) if state is None else state
+    outs = []
+    for t in range(x.shape[1]):
+        held = f[:, t] * h
+        if reset is not None:
+            held = torch.where(reset[:, t, None], torch.zeros_like(held), held)
+        h = held + v[:, t]
+        outs.append(h)
+    y = torch.stack(outs, 1).to(x.dtype) if outs else torch.empty_like(x)
+    return y, h if outs or state is None else h.clone()
+
+
+class _GatedRecurrenceFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, forget, input_gate, state, reset, forget_bias):
+        y, last, kept = ops.ext(required=True).gated_scan_fwd(x, forget, input_gate, state, reset, forget_bias, True)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, forget, input_gate, state, reset, kept)
+        ctx.forget_bias = forget_bias
+        return y, last
+
+    @staticmethod
+    def backward(ctx, dy, dlast):
+        x, forget, input_gate, state, reset, kept = ctx.saved_tensors
+        needed = ctx.needs_input_grad[:4]
+        if dy is None and dlast is None:
+            return (None,) * 6
+        if torch.is_grad_enabled():
+            grads = _differentiated_again(lambda *a: _scan_plain(*a, reset, ctx.forget_bias), (x, forget, input_gate, state), needed, (dy, dlast))
+        else:
+            dlast = None if dlast is None else dlast.float()
+            grads = ops.ext(required=True).gated_scan_bwd(dy, dlast, x, forget, input_gate, state, reset, kept, ctx.forget_bias)
+        return tuple(g if w else None for g, w in zip(grads, needed)) + (None, None)
+
+
+def gated_recurrence(x, forget, input_gate=None, state=None, reset=None, forget_bias=0.0):
+    """``h_t = f_t * h_{t-1} + u_t * x_t`` channel by channel over ``[batch, steps, channels]``: ``(h in x's type, last state in fp32)``.
+
+    ``f = sigmoid(forget + forget_bias)``; ``u = sigmoid(input_gate)``, or ``1 - f`` without one. ``state``: fp32 ``[batch, channels]``, the
+    state in front of the first step (zeros without one); pass the last state on to continue, one token at a time if need be.
+    ``reset``: bool ``[batch, steps]``, the steps that forget the state in front of them (a document begins). bf16 or fp32; strided views,
+    such as slices of one projection, are read in place. States are fp32 throughout; the backward pass computes them again."""
+    if x.dtype not in _STREAM_TYPES:
+        raise TypeError(f"gated_recurrence: bf16 or fp32 needed, got {x.dtype}")
+    if x.dim() != 3:
+        raise ValueError(f"gated_recurrence: [batch, steps, channels] needed, got {tuple(x.shape)}")
+    for t, what in ((forget, "forget gate"), (input_gate, "input gate")):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
+            raise ValueError(f"gated_recurrence: the {what} must have the input's shape and type, got {tuple(t.shape)} {t.dtype}")
+    if state is not None and (state.dtype != torch.float32 or state.shape != (x.shape[0], x.shape[2])):
+        raise ValueError(f"gated_recurrence: an fp32 state [batch, channels] needed, got {tuple(state.shape)} {state.dtype}")
+    if reset is not None and (reset.dtype != torch.bool or reset.shape != x.shape[:2]):
+        raise ValueError(f"gated_recurrence: a bool reset [batch, steps] needed, got {tuple(reset.shape)} {reset.dtype}")
+    if not _kernels(x):
+        return _scan_plain(x, forget, input_gate, state, reset, forget_bias)
+    if _wants_gradient(x, forget, input_gate, state):
+        return _GatedRecurrenceFn.apply(x, forget, input_gate, state, reset, float(forget_bias))
+    y, last, _ = ops.ext(required=True).gated_scan_fwd(x, forget, input_gate, state, reset, forget_bias, False)
+    return y, last
