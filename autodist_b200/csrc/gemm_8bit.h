@@ -5,8 +5,8 @@
 
 namespace adb200 {
 
-// y[m, n] = scales[m] * weight_scales[n] * sum_k codes[m, k] weight_codes[n, k] + bias[n], e4m3 codes, bf16 result. `*_ld`: elements (bytes)
-// between rows, multiples of 16, bases on 16 bytes.
+// y[m, n] = scales[m] * weight_scales[n] * sum_k codes[m, k] weight_codes[n, k] + bias[n], e4m3 codes, bf16 result. `*_ld`: bytes between rows, a
+// multiple of 16; codes, scales and bias start on 16-byte boundaries.
 struct Gemm8Args {
   const uint8_t* codes; long long codes_ld;
   const float* scales;
@@ -17,6 +17,7 @@ struct Gemm8Args {
   int M, N, K;
   int* error;                              // where a kernel that gave up waiting writes its code
 };
-cudaError_t gemm_8bit(const Gemm8Args& a, cudaStream_t st);
+// `bn`: rows of `codes` in a tile (16, 32, 64, 128; 512: the kernel on SM pairs), `split`: how many CTAs share a contraction (1 to 8); 0: chosen
+cudaError_t gemm_8bit(const Gemm8Args& a, int bn, int split, cudaStream_t st);
 
 }  // namespace adb200

@@ -171,9 +171,15 @@ Tensor aligned_codes(const Tensor& t, const char* what) {
   if (r.size(0) <= 1 && reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 == 0) return r;
   return empty_codes(r).copy_(r);
 }
+Tensor aligned_floats(const Tensor& t) {
+  const Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
+}
 int64_t code_stride(const Tensor& r) { return r.size(0) > 1 ? r.stride(0) : (r.size(1) + 15) / 16 * 16; }
 
-Tensor gemm_8bit(const Tensor& codes, const Tensor& scales, const Tensor& weight_codes, const Tensor& weight_scales, const optional<Tensor>& bias, Tensor error) {
+// `bn`, `split`: see gemm_8bit.h
+Tensor gemm_8bit(const Tensor& codes, const Tensor& scales, const Tensor& weight_codes, const Tensor& weight_scales, const optional<Tensor>& bias, Tensor error,
+                 int64_t bn, int64_t split) {
   const char* name = "linear_8bit";
   TORCH_CHECK(codes.is_cuda(), "linear_8bit: tensors on a GPU needed");
   check_gpu(codes, scales, name); check_gpu(codes, weight_codes, name); check_gpu(codes, weight_scales, name); check_gpu(codes, bias, name);
@@ -188,7 +194,7 @@ Tensor gemm_8bit(const Tensor& codes, const Tensor& scales, const Tensor& weight
               "linear_8bit: an fp32 scale for each row needed");
   TORCH_CHECK(!bias.has_value() || (bias->scalar_type() == at::kFloat && bias->numel() == N), "linear_8bit: an fp32 bias for each output needed");
   TORCH_CHECK(error.scalar_type() == at::kInt && error.numel() >= 1, "linear_8bit: an int32 word needed");
-  const Tensor sx = scales.contiguous(), sw = weight_scales.contiguous(), b = bias.has_value() ? bias->contiguous() : Tensor();
+  const Tensor sx = aligned_floats(scales), sw = aligned_floats(weight_scales), b = bias.has_value() ? aligned_floats(*bias) : Tensor();
   std::vector<int64_t> shape = codes.sizes().vec();
   shape.back() = N;
   Tensor y = at::empty(shape, codes.options().dtype(at::kBFloat16));
@@ -201,7 +207,7 @@ Tensor gemm_8bit(const Tensor& codes, const Tensor& scales, const Tensor& weight
   a.y = y.data_ptr();
   a.M = (int)M; a.N = (int)N; a.K = (int)x.size(1);
   a.error = error.data_ptr<int>();
-  launched(adb200::gemm_8bit(a, stream_of(codes)), name);
+  launched(adb200::gemm_8bit(a, (int)bn, (int)split, stream_of(codes)), name);
   return y;
 }
 
@@ -382,7 +388,8 @@ void register_lm(pybind11::module& m) {
   m.def("rms_norm_bwd", &rms_norm_bwd);
   m.def("rms_norm_8bit", &rms_norm_8bit);
   m.def("quantize_rows", &quantize_rows);
-  m.def("gemm_8bit", &gemm_8bit);
+  m.def("gemm_8bit", &gemm_8bit, py::arg("codes"), py::arg("scales"), py::arg("weight_codes"), py::arg("weight_scales"), py::arg("bias"), py::arg("error"),
+        py::arg("bn") = 0, py::arg("split") = 0);
   m.def("gated_scan_fwd", &gated_scan_fwd);
   m.def("gated_scan_bwd", &gated_scan_bwd);
   pybind11::class_<AdamwList, std::shared_ptr<AdamwList>>(m, "_AdamwList");

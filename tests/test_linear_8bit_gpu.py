@@ -56,6 +56,22 @@ def test_large(M, K, N):
     assert torch.equal(F.linear_8bit(*args), F.linear_8bit(*args))
 
 
+@pytest.mark.parametrize("bn", [16, 32, 64, 128, 512])
+@pytest.mark.parametrize("M,K,N", [(1, 1100, 130), (37, 2304, 264), (150, 1024, 1003), (300, 640, 520)])
+def test_every_tile_and_share(bn, M, K, N):
+    from autodist_b200 import ops
+    from autodist_b200.ops import functional as F
+    E, args = ops.ext(required=True), _inputs(M, K, N, bias=True)
+    err = F._error_flag(args[0].device)
+    for split in (1, 2, 3, 4, 5, 6, 7, 8) if bn != 512 else (1,):
+        if split <= (K + 127) // 128:
+            _check(args, E.gemm_8bit(*args, err, bn, split))
+        else:
+            with pytest.raises(RuntimeError, match="invalid"):
+                E.gemm_8bit(*args, err, bn, split)
+    F.check_errors()
+
+
 def test_codes_of_every_value():
     """All 256 codes: NaN rows give NaN, everything else its value."""
     from autodist_b200.ops import functional as F
@@ -167,6 +183,10 @@ def test_refusals():
     for bad in ((codes, scales[:4], weight, weight_scales), (codes, scales, weight, weight_scales.double()), (codes, scales[:, None], weight, weight_scales)):
         with pytest.raises(ValueError, match="scale for each row"):
             F.linear_8bit(*bad)
+    from autodist_b200 import ops
+    for bn, split in ((17, 1), (128, 9), (128, 2)):
+        with pytest.raises(RuntimeError, match="invalid"):
+            ops.ext(required=True).gemm_8bit(codes, scales, weight, weight_scales, None, F._error_flag(codes.device), bn, split)
     with pytest.raises(ValueError, match="bias"):
         F.linear_8bit(codes, scales, weight, weight_scales, bias.bfloat16())
     with pytest.raises(RuntimeError, match="no gradient"):
