@@ -229,7 +229,7 @@ ScanInputs scan_inputs(const Tensor& x, const Tensor& forget, const optional<Ten
   check_like(x, forget, name, "the forget gate");
   check_like(x, input, name, "the input gate");
   const int64_t B = x.size(0), T = x.size(1), C = x.size(2);
-  TORCH_CHECK(T < (1LL << 31) && B * ((C + 31) / 32) < (1LL << 31) / 64, "gated_recurrence: too large");
+  TORCH_CHECK(T < (1LL << 30) && B * ((C + 31) / 32) < (1LL << 31) / 64, "gated_recurrence: too large");
   in.a.x = scan_view(x, in.x);
   in.a.forget = scan_view(forget, in.forget);
   if (input.has_value()) in.a.input = scan_view(*input, in.input);

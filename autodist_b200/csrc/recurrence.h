@@ -5,7 +5,7 @@
 
 namespace adb200 {
 
-constexpr int kScanTile = 128;             // steps between the states that the forward pass keeps for the backward pass
+constexpr int kScanTile = 64;              // steps between the states that the forward pass keeps for the backward pass
 
 // [batch, steps, channels] views with unit stride along channels; strides in elements.
 struct ScanView { const void* p; long long batch, step; };
