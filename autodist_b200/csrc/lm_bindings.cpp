@@ -252,6 +252,11 @@ ScanInputs scan_inputs(const Tensor& x, const Tensor& forget, const optional<Ten
   return in;
 }
 
+int64_t kept_tiles(const adb200::ScanArgs& a) {
+  const int64_t tile = adb200::gated_scan_tile(a);
+  return (a.steps + tile - 1) / tile;
+}
+
 // -> (outputs, last state, states kept for the backward pass)
 std::tuple<Tensor, Tensor, optional<Tensor>> gated_scan_fwd(const Tensor& x, const Tensor& forget, const optional<Tensor>& input, const optional<Tensor>& state,
                                                             const optional<Tensor>& reset, double forget_bias, bool keep) {
@@ -260,7 +265,7 @@ std::tuple<Tensor, Tensor, optional<Tensor>> gated_scan_fwd(const Tensor& x, con
   ScanInputs in = scan_inputs(x, forget, input, state, reset, forget_bias);
   const auto f32 = x.options().dtype(at::kFloat);
   Tensor y = at::empty(x.sizes(), x.options()), last = at::empty({x.size(0), x.size(2)}, f32), kept;
-  if (keep) kept = at::empty({x.size(0), (x.size(1) + adb200::kScanTile - 1) / adb200::kScanTile, x.size(2)}, f32);
+  if (keep) kept = at::empty({x.size(0), kept_tiles(in.a), x.size(2)}, f32);
   launched(adb200::gated_scan_fwd(in.a, y.data_ptr(), last.data_ptr<float>(), keep ? kept.data_ptr<float>() : nullptr, stream_of(x)), "gated_recurrence");
   return {y, last, keep ? optional<Tensor>(kept) : c10::nullopt};
 }
@@ -275,7 +280,7 @@ std::tuple<Tensor, Tensor, optional<Tensor>, Tensor> gated_scan_bwd(const option
   check_like(x, dy, "gated_recurrence", "the gradient");
   const int64_t B = x.size(0), C = x.size(2);
   TORCH_CHECK(same_gpu(x, kept) && kept.scalar_type() == at::kFloat && kept.is_contiguous() &&
-                  kept.numel() == B * C * ((x.size(1) + adb200::kScanTile - 1) / adb200::kScanTile), "gated_recurrence: the forward pass's states needed");
+                  kept.numel() == B * C * kept_tiles(in.a), "gated_recurrence: the forward pass's states needed");
   adb200::ScanGrads g{};
   Tensor dy_held, dlast_held;
   if (dy.has_value()) g.dy = scan_view(*dy, dy_held);

@@ -5,8 +5,6 @@
 
 namespace adb200 {
 
-constexpr int kScanTile = 64;              // steps between the states that the forward pass keeps for the backward pass
-
 // [batch, steps, channels] views with unit stride along channels; strides in elements.
 struct ScanView { const void* p; long long batch, step; };
 struct ScanArgs {
@@ -17,8 +15,10 @@ struct ScanArgs {
   float forget_bias;
   bool bf16;                               // else fp32
 };
-// y: [batch, steps, channels], last: [batch, channels]; kept (nullptr: not wanted): [batch, ceil(steps / kScanTile), channels], the states in front
-// of each tile
+// Steps between the states that the forward pass keeps for the backward pass; goes by the sizes alone.
+int gated_scan_tile(const ScanArgs& a);
+// y: [batch, steps, channels], last: [batch, channels]; kept (nullptr: not wanted): [batch, ceil(steps / gated_scan_tile), channels], the states
+// in front of each tile
 cudaError_t gated_scan_fwd(const ScanArgs& a, void* y, float* last, float* kept, cudaStream_t st);
 
 struct ScanGrads {

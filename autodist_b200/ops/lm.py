@@ -4,6 +4,8 @@ linear recurrence over time, and the product of 8-bit rows.
 CUDA tensors run on the hand-written kernels, CPU tensors on the plain PyTorch expressions below, which are also what second
 derivatives, forward-mode derivatives and ``torch.func`` transforms go through.
 """
+import math
+
 import torch
 import torch.nn.functional as F
 
@@ -204,6 +206,8 @@ def gated_recurrence(x, forget, input_gate=None, state=None, reset=None, forget_
         raise ValueError(f"gated_recurrence: an fp32 state [batch, channels] needed, got {tuple(state.shape)} {state.dtype}")
     if reset is not None and (reset.dtype != torch.bool or reset.shape != x.shape[:2]):
         raise ValueError(f"gated_recurrence: a bool reset [batch, steps] needed, got {tuple(reset.shape)} {reset.dtype}")
+    if not math.isfinite(forget_bias):
+        raise ValueError(f"gated_recurrence: a finite forget_bias needed, got {forget_bias}")
     if not _kernels(x):
         return _scan_plain(x, forget, input_gate, state, reset, forget_bias)
     if _wants_gradient(x, forget, input_gate, state):

@@ -309,6 +309,9 @@ def test_refusals():
     for args in ((x, x.cpu()), (x, x, None, state.cpu()), (x, x, None, None, reset.cpu())):
         with pytest.raises(RuntimeError, match="GPU"):
             F.gated_recurrence(*args)
+    for bad in (float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="finite forget_bias"):
+            F.gated_recurrence(x, x, forget_bias=bad)
     E = ops.ext(required=True)
     with pytest.raises(RuntimeError, match="GPU"):
         E.gated_scan_fwd(x.cpu(), x, None, None, None, 0.0, False)
