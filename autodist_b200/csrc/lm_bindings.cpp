@@ -257,8 +257,13 @@ int64_t kept_tiles(const adb200::ScanArgs& a) {
   return (a.steps + tile - 1) / tile;
 }
 
-// -> (outputs, last state, states kept for the backward pass)
-std::tuple<Tensor, Tensor, optional<Tensor>> gated_scan_fwd(const Tensor& x, const Tensor& forget, const optional<Tensor>& input, const optional<Tensor>& state,
+Tensor scan_scratch(const adb200::ScanArgs& a, const at::TensorOptions& f32) {
+  const long long n = adb200::gated_scan_runs(a);
+  return n > 0 ? at::empty({n}, f32) : Tensor();
+}
+
+// -> (outputs, last state, states kept for the backward pass, kernels launched)
+std::tuple<Tensor, Tensor, optional<Tensor>, int> gated_scan_fwd(const Tensor& x, const Tensor& forget, const optional<Tensor>& input, const optional<Tensor>& state,
                                                             const optional<Tensor>& reset, double forget_bias, bool keep) {
   TORCH_CHECK(x.is_cuda(), "gated_recurrence: tensors on a GPU needed");
   const c10::cuda::CUDAGuard guard(x.device());
@@ -266,12 +271,15 @@ std::tuple<Tensor, Tensor, optional<Tensor>> gated_scan_fwd(const Tensor& x, con
   const auto f32 = x.options().dtype(at::kFloat);
   Tensor y = at::empty(x.sizes(), x.options()), last = at::empty({x.size(0), x.size(2)}, f32), kept;
   if (keep) kept = at::empty({x.size(0), kept_tiles(in.a), x.size(2)}, f32);
-  launched(adb200::gated_scan_fwd(in.a, y.data_ptr(), last.data_ptr<float>(), keep ? kept.data_ptr<float>() : nullptr, stream_of(x)), "gated_recurrence");
-  return {y, last, keep ? optional<Tensor>(kept) : c10::nullopt};
+  const Tensor runs = scan_scratch(in.a, f32);
+  int kernels = 0;
+  launched(adb200::gated_scan_fwd(in.a, y.data_ptr(), last.data_ptr<float>(), keep ? kept.data_ptr<float>() : nullptr, runs.defined() ? runs.data_ptr<float>() : nullptr,
+                                  &kernels, stream_of(x)), "gated_recurrence");
+  return {y, last, keep ? optional<Tensor>(kept) : c10::nullopt, kernels};
 }
 
-// -> gradients of (x, forget, input, state)
-std::tuple<Tensor, Tensor, optional<Tensor>, Tensor> gated_scan_bwd(const optional<Tensor>& dy, const optional<Tensor>& dlast, const Tensor& x, const Tensor& forget,
+// -> gradients of (x, forget, input, state), kernels launched
+std::tuple<Tensor, Tensor, optional<Tensor>, Tensor, int> gated_scan_bwd(const optional<Tensor>& dy, const optional<Tensor>& dlast, const Tensor& x, const Tensor& forget,
                                                                     const optional<Tensor>& input, const optional<Tensor>& state, const optional<Tensor>& reset,
                                                                     const Tensor& kept, double forget_bias) {
   TORCH_CHECK(x.is_cuda(), "gated_recurrence: tensors on a GPU needed");
@@ -293,8 +301,10 @@ std::tuple<Tensor, Tensor, optional<Tensor>, Tensor> gated_scan_bwd(const option
   if (input.has_value()) dinput = at::empty(x.sizes(), x.options());
   g.kept = kept.data_ptr<float>();
   g.dx = dx.data_ptr(); g.dforget = dforget.data_ptr(); g.dinput = input.has_value() ? dinput.data_ptr() : nullptr; g.dstate = dstate.data_ptr<float>();
-  launched(adb200::gated_scan_bwd(in.a, g, stream_of(x)), "gated_recurrence");
-  return {dx, dforget, input.has_value() ? optional<Tensor>(dinput) : c10::nullopt, dstate};
+  const Tensor runs = scan_scratch(in.a, kept.options());
+  int kernels = 0;
+  launched(adb200::gated_scan_bwd(in.a, g, runs.defined() ? runs.data_ptr<float>() : nullptr, &kernels, stream_of(x)), "gated_recurrence");
+  return {dx, dforget, input.has_value() ? optional<Tensor>(dinput) : c10::nullopt, dstate, kernels};
 }
 
 // ---------------------------------------------------------------------------------------------- optimizer

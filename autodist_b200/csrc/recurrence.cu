@@ -13,8 +13,9 @@
 //   a warp          walks along its sequence alone where there are enough of them; its inputs come ahead of it into a ring of its own in
 //                   shared memory (cp.async), so that a wait of one warp holds up no other
 //   a thread block  of up to 8 warps takes as many runs of steps side by side, joined through shared memory, where there are fewer channels
-//   a cluster       of S blocks takes S such tiles at once where there are fewer still: each block writes its (A, H) into the others'
-//                   shared memory, one cluster barrier a round. Nothing spins on global memory; the order of joining is fixed.
+//   chunks          of the sequence go to blocks of their own where there are fewer still. What the chunks do is computed first, by a kernel
+//                   whose warps hear from nobody (the inputs are read twice, but by as many blocks as the GPU holds); a chunk's block
+//                   folds those in front of its own. The order of joining is fixed.
 //
 // The states are not stored: the forward pass keeps them in fp32 in front of every tile of the backward pass, which walks the other way with
 // the same joining of dh and computes those in between again. States, gates and sums are fp32.
@@ -23,10 +24,11 @@
 #include <cuda_bf16.h>
 
 #include <initializer_list>
+#include <type_traits>
 
-#include "pair_tcgen05.cuh"
 #include "pdl.cuh"
 #include "sm_count.h"
+#include "tcgen05_common.cuh"
 
 namespace adb200 {
 namespace {
@@ -34,7 +36,7 @@ namespace {
 typedef __nv_bfloat16 bf16;
 constexpr int kWarps = 8;                    // of a block at most
 constexpr int kBack = 8;                     // steps of a warp in the backward pass
-constexpr int kMostSplit = 16;
+constexpr int kLeastTiles = 2;               // of a chunk
 
 // fp32 values of a lane's channels, one or two of them; two take one instruction.
 template <int VEC> struct F;
@@ -143,27 +145,20 @@ template <bool CUT, int VEC> __device__ __forceinline__ Run<VEC> joined(const Ru
   return {a, after<CUT>(then, first.b)};
 }
 
-__device__ __forceinline__ void store_cluster(uint32_t addr, Run<1> r) {
-  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(r.a.v), "f"(r.b.v) : "memory");
-}
-__device__ __forceinline__ void store_cluster(uint32_t addr, Run<2> r) {
-  asm volatile("st.shared::cluster.v2.b64 [%0], {%1, %2};" ::"r"(addr), "l"(r.a.v), "l"(r.b.v) : "memory");
-}
-
 // Where a thread works. `warps`: warps of a tile; a block holds kWarps / warps tiles of neighbouring channel groups, or one.
 template <int VEC>
 struct Place {
   int lane, warp, part, first;               // part: the warp's place in its tile, whose first warp is `first`
-  int b, c0, c, rank;                        // c0: the warp's first channel
+  int b, c0, c, chunk;                       // c0: the warp's first channel
   bool live;
-  __device__ __forceinline__ Place(const ScanArgs& a, int warps, int split) {
+  __device__ __forceinline__ Place(const ScanArgs& a, int warps, int chunks) {
     lane = threadIdx.x & 31;
     warp = threadIdx.x >> 5;
     part = warp % warps;
     first = warp - part;
-    rank = split > 1 ? (int)tc::cluster_ctarank() : 0;
+    chunk = blockIdx.x % chunks;
     const int across = (a.channels + 32 * VEC - 1) / (32 * VEC);
-    const int column = blockIdx.x / split * (blockDim.x / 32 / warps) + warp / warps;
+    const int column = blockIdx.x / chunks * (blockDim.x / 32 / warps) + warp / warps;
     b = column / across;
     c0 = column % across * 32 * VEC;
     c = c0 + lane * VEC;
@@ -184,47 +179,61 @@ struct Ring {
   typedef typename Lane<T, VEC>::Raw Raw;
   static constexpr int ROW = 32 * VEC * (int)sizeof(T);
   static constexpr int SLOT = NT * STEPS * ROW;
-  static constexpr int FIT = 84 * 1024 / (kWarps * SLOT);       // two blocks and what they exchange through on an SM
+  static constexpr int FIT = 94 * 1024 / (kWarps * SLOT);       // two blocks and what they exchange through on an SM
   static constexpr int SLOTS = FIT < 2 ? 2 : FIT > 4 ? 4 : FIT;
   static constexpr int BYTES = SLOTS * SLOT;             // of a warp
 };
 
-// Requests one tensor's rows t0 ... of a warp's channels; rows and channels that are not there hold `none`. `wide`: whole 16-byte pieces.
+// One tensor's rows of a warp, from which it requests a tile after the other. `wide`: whole 16-byte pieces, else a lane's channels by itself.
 template <typename T, int VEC, int STEPS>
-__device__ __forceinline__ void request_rows(uint8_t* dst, const ScanView& v, int b, int t0, int rows, int c0, int channels, int lane, bool wide,
-                                             typename Lane<T, VEC>::Raw none) {
+struct Source {
   typedef typename Lane<T, VEC>::Raw Raw;
-  constexpr int ROW = 32 * VEC * (int)sizeof(T), PIECES = ROW / 16, PER = 32 / PIECES;
-  const T* base = static_cast<const T*>(v.p) + b * v.batch + t0 * v.step + c0;
-  if (wide) {
-    const int piece = lane % PIECES, c = piece * (16 / (int)sizeof(T));
-    const T* src = base + lane / PIECES * v.step + c;
-    uint8_t* to = dst + lane * 16;
-    const int left = c0 + c < channels ? rows - lane / PIECES : 0;
+  static constexpr int ROW = 32 * VEC * (int)sizeof(T), PIECES = ROW / 16, PER = 32 / PIECES;
+  static_assert(STEPS % PER == 0, "whole rounds of pieces");
+  const T* src;                              // what this lane copies first
+  long long step, advance;                   // from a step to the next, and from a request to the next
+  __device__ __forceinline__ Source(const ScanView& v, int b, int t0, int c0, int lane, bool wide, int steps_between) {
+    src = static_cast<const T*>(v.p) + b * v.batch + t0 * v.step + c0 + (wide ? lane / PIECES * v.step + lane % PIECES * (16 / (int)sizeof(T)) : lane * VEC);
+    step = v.step;
+    advance = steps_between * v.step;
+  }
+  // Rows and channels that are not there hold `none`. `full`: all of them are.
+  __device__ __forceinline__ void request(uint8_t* dst, int rows, int channels, int lane, bool wide, bool full, Raw none) {
+    const T* from = src;
+    src += advance;
+    if (wide && full) {
+      const uint32_t to = tc::smem_u32(dst) + (uint32_t)lane * 16u;
 #pragma unroll
-    for (int i = 0; i < (STEPS + PER - 1) / PER; ++i, src += PER * v.step, to += 512) {
-      if (STEPS % PER != 0 && i * PER + lane / PIECES >= STEPS) break;
-      if (i * PER < left) {
-        copy_async<16>(tc::smem_u32(to), src);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 16 / (int)sizeof(Raw); ++j) reinterpret_cast<Raw*>(to)[j] = none;
+      for (int i = 0; i < STEPS / PER; ++i, from += PER * step) copy_async<16>(to + i * 512u, from);
+    } else if (wide) {
+      uint8_t* to = dst + lane * 16;
+      const int left = lane % PIECES * (16 / (int)sizeof(T)) < channels ? rows - lane / PIECES : 0;
+#pragma unroll 1
+      for (int i = 0; i < STEPS / PER; ++i, from += PER * step, to += 512) {
+        if (i * PER < left) {
+          copy_async<16>(tc::smem_u32(to), from);
+        } else {
+          for (int j = 0; j < 16 / (int)sizeof(Raw); ++j) reinterpret_cast<Raw*>(to)[j] = none;
+        }
       }
-    }
-  } else {
-    const T* src = base + lane * VEC;
-    Raw* to = reinterpret_cast<Raw*>(dst) + lane;
-    const int left = c0 + lane * VEC < channels ? rows : 0;
+    } else {
+      Raw* to = reinterpret_cast<Raw*>(dst) + lane;
+      const int left = lane * VEC < channels ? rows : 0;
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i, src += v.step, to += 32) {
-      if (i < left) {
-        if constexpr (sizeof(Raw) >= 4) copy_async<sizeof(Raw)>(tc::smem_u32(to), src);
-        else *to = *reinterpret_cast<const Raw*>(src);
-      } else {
-        *to = none;
+      for (int i = 0; i < STEPS; ++i, from += step, to += 32) {
+        if (i < left) {
+          if constexpr (sizeof(Raw) >= 4) copy_async<sizeof(Raw)>(tc::smem_u32(to), from);
+          else *to = *reinterpret_cast<const Raw*>(from);
+        } else {
+          *to = none;
+        }
       }
     }
   }
+};
+// A lane's place in rows that are `row` bytes apart.
+template <typename T> __device__ __forceinline__ T* row_at(T* p, uint32_t row, uint32_t i) {
+  return reinterpret_cast<T*>(reinterpret_cast<char*>(p) + (uint64_t)row * i);
 }
 // Bit i: the state in front of step t0 + i is forgotten.
 template <int STEPS>
@@ -233,30 +242,130 @@ __device__ __forceinline__ uint32_t load_cuts(const ScanArgs& a, int b, int t0, 
   return __ballot_sync(0xffffffffu, cut);
 }
 
+// Chunks of `tiles` tiles each that a sequence is cut into. runs: what the `pieces` of each do to a state (forward) or to dh (backward),
+// [count * pieces][2][batch][channels].
+struct Chunks {
+  int count, tiles, pieces;
+  float* runs;
+  template <int VEC> __device__ __forceinline__ Run<VEC> run(const ScanArgs& a, int z, long long state_at) const {
+    const long long plane = (long long)a.batch * a.channels;
+    const float* p = runs + 2LL * z * plane + state_at;
+    return {load_f(p, static_cast<F<VEC>*>(nullptr)), load_f(p + plane, static_cast<F<VEC>*>(nullptr))};
+  }
+};
+
+// What each piece of each chunk but the last (backward: but the first) does: its steps in equal runs, a warp each.
+template <typename T, int VEC, bool GATE, bool CUT, bool BACK>
+__global__ void __launch_bounds__(32 * kWarps, 3)
+scan_chunks_kernel(const ScanArgs a, const ScanView dy, const int wide, const int tile_steps, const Chunks ch) {
+  typedef Lane<T, VEC> L;
+  constexpr int STEPS = kBack;
+  constexpr bool INPUT = GATE && !BACK;
+  typedef Ring<T, VEC, STEPS, INPUT ? 3 : 2> R;
+  extern __shared__ __align__(16) uint8_t ring_all[];
+  __shared__ Run<VEC> parts[kWarps][32];
+  pdl_sync();
+  const Place<VEC> at(a, kWarps, (ch.count - 1) * ch.pieces);
+  const int chunk = at.chunk / ch.pieces + (BACK ? 1 : 0), piece = at.chunk % ch.pieces, z = chunk * ch.pieces + piece;
+  const int tile0 = ch.tiles * piece / ch.pieces, run_steps = (ch.tiles * (piece + 1) / ch.pieces - tile0) * tile_steps / kWarps;
+  const int t_first = (chunk * ch.tiles + tile0) * tile_steps + at.warp * run_steps, rounds = run_steps / STEPS;
+  const int channels = a.channels - at.c0;
+  uint8_t* ring = ring_all + at.warp * R::BYTES;
+  Source<T, VEC, STEPS> from_forget(a.forget, at.b, t_first, at.c0, at.lane, wide, STEPS), from_value(BACK ? dy : a.x, at.b, t_first, at.c0, at.lane, wide, STEPS),
+      from_input(a.input, at.b, t_first, at.c0, at.lane, wide, STEPS);
+  int rows = a.steps - t_first;
+  auto request = [&](int k) {
+    if (k < rounds) {
+      uint8_t* slot = ring + k % R::SLOTS * R::SLOT;
+      const bool full = rows >= STEPS && channels >= 32 * VEC, value = !BACK || dy.p != nullptr;
+      from_forget.request(slot, rows, channels, at.lane, wide, full, L::kOpen);
+      from_value.request(slot + STEPS * R::ROW, value ? rows : 0, channels, at.lane, wide, full && value, 0);
+      if constexpr (INPUT) from_input.request(slot + 2 * STEPS * R::ROW, rows, channels, at.lane, wide, full, 0);
+      rows -= STEPS;
+    }
+    commit_copies();
+  };
+#pragma unroll
+  for (int k = 0; k < R::SLOTS - 1; ++k) request(k);
+  const Gate<T, VEC> forget(a.forget_bias), input(0.f);
+  uint32_t cuts = 0, next_cuts = 0;
+  if (CUT) next_cuts = load_cuts<STEPS>(a, at.b, t_first, at.lane);
+  Run<VEC> sum = {all<VEC>(1.f), all<VEC>(0.f)};
+  for (int k = 0; k < rounds; ++k) {
+    request(k + R::SLOTS - 1);
+    wait_copies<R::SLOTS - 1>();
+    __syncwarp();
+    if (CUT) {
+      cuts = next_cuts;
+      if (k + 1 < rounds) next_cuts = load_cuts<STEPS>(a, at.b, t_first + (k + 1) * STEPS, at.lane);
+    }
+    const typename L::Raw* raw = reinterpret_cast<const typename L::Raw*>(ring + k % R::SLOTS * R::SLOT) + at.lane;
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      F<VEC> f, n;
+      forget(L::unpack(raw[i * 32]), f, n);
+      if constexpr (INPUT) {
+        F<VEC> m;
+        input(L::unpack(raw[(2 * STEPS + i) * 32]), n, m);
+      }
+      const F<VEC> value = L::unpack(raw[(STEPS + i) * 32]);
+      const bool cut = CUT && (cuts >> i & 1);
+      if (BACK) {                              // f_0 (dy_0 + f_1 (dy_1 + ...)), summed from the front
+        sum.a = mul(sum.a, f);
+        if (cut) sum.a = all<VEC>(-0.f);
+        const F<VEC> more = fma(sum.a, value, sum.b);
+        sum.b = CUT ? where_cut(sum.a, sum.b, more) : more;
+      } else {
+        const F<VEC> w = mul(n, value);
+        sum = {mul(sum.a, f), fma(f, sum.b, w)};
+        if (cut) sum = {all<VEC>(-0.f), w};
+      }
+    }
+    __syncwarp();                              // the slot has been read
+  }
+  wait_copies<0>();
+  parts[at.warp][at.lane] = sum;
+  __syncthreads();
+  if (at.warp == 0 && at.live) {
+    Run<VEC> whole = parts[BACK ? kWarps - 1 : 0][at.lane];
+#pragma unroll
+    for (int j = 1; j < kWarps; ++j) whole = joined<CUT>(whole, parts[BACK ? kWarps - 1 - j : j][at.lane]);
+    const long long plane = (long long)a.batch * a.channels;
+    float* p = ch.runs + 2LL * z * plane + (long long)at.b * a.channels + at.c;
+    store_f(p, whole.a);
+    store_f(p + plane, whole.b);
+  }
+}
+
 template <typename T, int VEC, bool GATE, bool CUT, int STEPS>
 __global__ void __launch_bounds__(32 * kWarps, 2)
-scan_fwd_kernel(const ScanArgs a, T* __restrict__ y, float* __restrict__ last, float* __restrict__ kept, const int keep, const int wide, const int warps,
-                const int split) {
+scan_fwd_kernel(const ScanArgs a, T* __restrict__ y, float* __restrict__ last, float* __restrict__ kept, const int keep_log2, const int wide,
+                const int warps, const Chunks ch) {
   typedef Lane<T, VEC> L;
   typedef F<VEC> V;
   typedef Ring<T, VEC, STEPS, GATE ? 3 : 2> R;
   extern __shared__ __align__(16) uint8_t ring_all[];
   __shared__ Run<VEC> parts[2][kWarps][32];
-  __shared__ Run<VEC> tiles[2][kMostSplit][32];
+  __shared__ V carries[2][kWarps][32];         // the state behind a tile
   pdl_sync();
-  const Place<VEC> at(a, warps, split);
+  const Place<VEC> at(a, warps, ch.count);
   const int tile_steps = warps * STEPS;
-  const int count = (a.steps + tile_steps - 1) / tile_steps, rounds = (count + split - 1) / split;
+  const int count = (a.steps + tile_steps - 1) / tile_steps, tile0 = at.chunk * ch.tiles, rounds = min(ch.tiles, count - tile0);
   uint8_t* ring = ring_all + at.warp * R::BYTES;
   const bool there = at.b < a.batch;
+  const int t_first = tile0 * tile_steps + at.part * STEPS;
+  const int channels = there ? a.channels - at.c0 : 0;         // of this warp, from its first on
+  Source<T, VEC, STEPS> from_forget(a.forget, at.b, t_first, at.c0, at.lane, wide, tile_steps), from_x(a.x, at.b, t_first, at.c0, at.lane, wide, tile_steps),
+      from_input(a.input, at.b, t_first, at.c0, at.lane, wide, tile_steps);
+  int request_rows = a.steps - t_first;
   auto request = [&](int k) {
-    const int t0 = (k * split + at.rank) * tile_steps + at.part * STEPS;
     if (k < rounds) {
       uint8_t* slot = ring + k % R::SLOTS * R::SLOT;
-      const int rows = there ? a.steps - t0 : 0;
-      request_rows<T, VEC, STEPS>(slot, a.forget, at.b, t0, rows, at.c0, a.channels, at.lane, wide, L::kOpen);
-      request_rows<T, VEC, STEPS>(slot + STEPS * R::ROW, a.x, at.b, t0, rows, at.c0, a.channels, at.lane, wide, 0);
-      if constexpr (GATE) request_rows<T, VEC, STEPS>(slot + 2 * STEPS * R::ROW, a.input, at.b, t0, rows, at.c0, a.channels, at.lane, wide, 0);
+      const bool full = request_rows >= STEPS && channels >= 32 * VEC;
+      from_forget.request(slot, request_rows, channels, at.lane, wide, full, L::kOpen);
+      from_x.request(slot + STEPS * R::ROW, request_rows, channels, at.lane, wide, full, 0);
+      if constexpr (GATE) from_input.request(slot + 2 * STEPS * R::ROW, request_rows, channels, at.lane, wide, full, 0);
+      request_rows -= tile_steps;
     }
     commit_copies();
   };
@@ -264,19 +373,21 @@ scan_fwd_kernel(const ScanArgs a, T* __restrict__ y, float* __restrict__ last, f
   for (int k = 0; k < R::SLOTS - 1; ++k) request(k);
   const long long state_at = (long long)at.b * a.channels + at.c;
   V carry = at.live && a.state != nullptr ? load_f(a.state + state_at, static_cast<V*>(nullptr)) : all<VEC>(0.f);
+  if (at.live)
+#pragma unroll 4
+    for (int z = 0; z < at.chunk * ch.pieces; ++z) carry = after<CUT>(ch.run<VEC>(a, z, state_at), carry);
   const Gate<T, VEC> forget(a.forget_bias), input(0.f);
   uint32_t cuts = 0, next_cuts = 0;
-  if (CUT) next_cuts = load_cuts<STEPS>(a, at.b, at.rank * tile_steps + at.part * STEPS, at.lane);
-  if (split > 1) tc::cluster_sync_all();       // the others' shared memory is there
+  if (CUT) next_cuts = load_cuts<STEPS>(a, at.b, t_first, at.lane);
 
   for (int k = 0; k < rounds; ++k) {
-    const int tile = k * split + at.rank, t0 = tile * tile_steps + at.part * STEPS, buf = k & 1;
+    const int t0 = t_first + k * tile_steps, buf = k & 1;
     request(k + R::SLOTS - 1);
     wait_copies<R::SLOTS - 1>();
     __syncwarp();
     if (CUT) {
       cuts = next_cuts;
-      if (k + 1 < rounds) next_cuts = load_cuts<STEPS>(a, at.b, t0 + split * tile_steps, at.lane);
+      if (k + 1 < rounds) next_cuts = load_cuts<STEPS>(a, at.b, t0 + tile_steps, at.lane);
     }
     const typename L::Raw* raw = reinterpret_cast<const typename L::Raw*>(ring + k % R::SLOTS * R::SLOT) + at.lane;
     V f[STEPS], w[STEPS];
@@ -295,107 +406,99 @@ scan_fwd_kernel(const ScanArgs a, T* __restrict__ y, float* __restrict__ last, f
       if (CUT && (cuts >> i & 1)) sum = {all<VEC>(-0.f), w[i]};
     }
     __syncwarp();                              // the slot has been read
+    V start = carry;
     if (warps > 1) {
       parts[buf][at.warp][at.lane] = sum;
       __syncthreads();
-    }
-    V h = carry;
-    if (split > 1) {
-      // the tile as a whole, to every block of the cluster
-      Run<VEC> whole = parts[buf][0][at.lane];
-#pragma unroll
-      for (int j = 1; j < kWarps; ++j) whole = joined<CUT>(whole, parts[buf][j][at.lane]);
-      for (int r = at.warp; r < split; r += kWarps) store_cluster(tc::map_to_cta(tc::smem_u32(&tiles[buf][at.rank][at.lane]), (uint32_t)r), whole);
-      __syncwarp();
-      tc::cluster_sync_all();
-      V front = h;
+      if (k > 0) start = carries[buf ^ 1][at.first][at.lane];
 #pragma unroll 4
-      for (int r = 0; r < split; ++r) {
-        if (r == at.rank) front = h;
-        h = after<CUT>(tiles[buf][r][at.lane], h);
-      }
-      carry = h;
-      h = front;
+      for (int j = 0; j < at.part; ++j) start = after<CUT>(parts[buf][at.first + j][at.lane], start);
+      carry = after<CUT>(sum, start);          // the last warp knows what the next tile starts from
+      if (at.part == warps - 1) carries[buf][at.first][at.lane] = carry;
+    } else {
+      carry = after<CUT>(sum, start);
     }
-    V start = h;
-    if (warps == kWarps) {
+    const int rows = at.live ? a.steps - t0 : 0;
+    // states in front of the backward pass's tiles
+    auto keep_state = [&](int t, V h) {
+      store_f(kept + ((long long)at.b * ((a.steps + (1 << keep_log2) - 1) >> keep_log2) + (t >> keep_log2)) * a.channels + at.c, h);
+    };
+    const bool keeps = kept != nullptr && (t0 & ((1 << keep_log2) - 1)) == 0;
+    if (keeps && rows > 0) keep_state(t0, start);
+    T* out = y + ((long long)at.b * a.steps + t0) * a.channels + at.c;
+    const uint32_t row = (uint32_t)a.channels * (uint32_t)sizeof(T);
+    V h = start;
+    if (rows >= STEPS && !(STEPS > kBack && keeps && (1 << keep_log2) == kBack)) {
 #pragma unroll
-      for (int j = 0; j < kWarps; ++j) {
-        if (j == at.part) start = h;
-        h = after<CUT>(parts[buf][j][at.lane], h);
-      }
-    } else if (warps > 1) {
-      for (int j = 0; j < warps; ++j) {
-        if (j == at.part) start = h;
-        h = after<CUT>(parts[buf][at.first + j][at.lane], h);
+      for (int i = 0; i < STEPS; ++i) {
+        h = CUT && (cuts >> i & 1) ? w[i] : fma(f[i], h, w[i]);
+        L::store(row_at(out, row, i), h);
       }
     } else {
-      h = after<CUT>(sum, h);
-    }
-    if (split == 1) carry = h;
-    const int rows = at.live ? a.steps - t0 : 0;
-    // states in front of the backward pass's tiles, whose length is a multiple of this warp's steps, or half of them
-    if (kept != nullptr && rows > 0) {
-      if (t0 % keep == 0) store_f(kept + ((long long)at.b * ((a.steps + keep - 1) / keep) + t0 / keep) * a.channels + at.c, start);
-    }
-    T* out = y + ((long long)at.b * a.steps + t0) * a.channels + at.c;
-    h = start;
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i, out += a.channels) {
-      if (STEPS > kBack && i == kBack && kept != nullptr && keep == kBack && i < rows)
-        store_f(kept + ((long long)at.b * ((a.steps + keep - 1) / keep) + (t0 + i) / keep) * a.channels + at.c, h);
-      h = CUT && (cuts >> i & 1) ? w[i] : fma(f[i], h, w[i]);
-      if (i < rows) L::store(out, h);
+      for (int i = 0; i < STEPS; ++i) {
+        if (STEPS > kBack && i == kBack && keeps && (1 << keep_log2) == kBack && i < rows) keep_state(t0 + i, h);
+        h = CUT && (cuts >> i & 1) ? w[i] : fma(f[i], h, w[i]);
+        if (i < rows) L::store(row_at(out, row, i), h);
+      }
     }
   }
   wait_copies<0>();
-  if (at.rank == 0 && at.part == 0 && at.live) store_f(last + state_at, carry);
+  if (at.chunk == ch.count - 1 && at.part == warps - 1 && at.live) store_f(last + state_at, carry);
 }
 
 template <typename T, int VEC, bool GATE, bool CUT>
 __global__ void __launch_bounds__(32 * kWarps, 2)
-scan_bwd_kernel(const ScanArgs a, const ScanGrads g, const int wide, const int warps, const int split) {
+scan_bwd_kernel(const ScanArgs a, const ScanGrads g, const int wide, const int warps, const Chunks ch) {
   typedef Lane<T, VEC> L;
   typedef F<VEC> V;
   constexpr int STEPS = kBack;
   typedef Ring<T, VEC, STEPS, GATE ? 4 : 3> R;
   extern __shared__ __align__(16) uint8_t ring_all[];
   __shared__ Run<VEC> parts[2][kWarps][32];              // of a warp's steps
+  __shared__ V carries[2][kWarps][32];                   // f dh in front of a tile
   __shared__ V back[2][kWarps][32];                      // their dh: from the end of the steps to their front it is a dh + back
-  __shared__ Run<VEC> tiles[2][kMostSplit][32];          // a and back of a tile
   pdl_sync();
-  const Place<VEC> at(a, warps, split);
+  const Place<VEC> at(a, warps, ch.count);
   const int tile_steps = warps * STEPS;
-  const int count = (a.steps + tile_steps - 1) / tile_steps, rounds = (count + split - 1) / split;
+  const int count = (a.steps + tile_steps - 1) / tile_steps, tile0 = at.chunk * ch.tiles, rounds = min(ch.tiles, count - tile0);
   uint8_t* ring = ring_all + at.warp * R::BYTES;
   const bool there = at.b < a.batch;
   // rounds are counted from the last tiles to the first
-  auto t0_of = [&](int k) { return ((rounds - 1 - k) * split + at.rank) * tile_steps + at.part * STEPS; };
+  auto t0_of = [&](int k) { return (tile0 + rounds - 1 - k) * tile_steps + at.part * STEPS; };
+  const int t_first = t0_of(0);
+  const int channels = there ? a.channels - at.c0 : 0;         // of this warp, from its first on
+  Source<T, VEC, STEPS> from_forget(a.forget, at.b, t_first, at.c0, at.lane, wide, -tile_steps), from_x(a.x, at.b, t_first, at.c0, at.lane, wide, -tile_steps),
+      from_dy(g.dy, at.b, t_first, at.c0, at.lane, wide, -tile_steps), from_input(a.input, at.b, t_first, at.c0, at.lane, wide, -tile_steps);
+  int request_rows = a.steps - t_first;
   auto request = [&](int k) {
     if (k < rounds) {
-      const int t0 = t0_of(k), rows = there ? a.steps - t0 : 0;
       uint8_t* slot = ring + k % R::SLOTS * R::SLOT;
-      request_rows<T, VEC, STEPS>(slot, a.forget, at.b, t0, rows, at.c0, a.channels, at.lane, wide, L::kOpen);
-      request_rows<T, VEC, STEPS>(slot + STEPS * R::ROW, a.x, at.b, t0, rows, at.c0, a.channels, at.lane, wide, 0);
-      request_rows<T, VEC, STEPS>(slot + 2 * STEPS * R::ROW, g.dy, at.b, t0, g.dy.p != nullptr ? rows : 0, at.c0, a.channels, at.lane, wide, 0);
-      if constexpr (GATE) request_rows<T, VEC, STEPS>(slot + 3 * STEPS * R::ROW, a.input, at.b, t0, rows, at.c0, a.channels, at.lane, wide, 0);
+      const bool full = request_rows >= STEPS && channels >= 32 * VEC, dy = g.dy.p != nullptr;
+      from_forget.request(slot, request_rows, channels, at.lane, wide, full, L::kOpen);
+      from_x.request(slot + STEPS * R::ROW, request_rows, channels, at.lane, wide, full, 0);
+      from_dy.request(slot + 2 * STEPS * R::ROW, dy ? request_rows : 0, channels, at.lane, wide, full && dy, 0);
+      if constexpr (GATE) from_input.request(slot + 3 * STEPS * R::ROW, request_rows, channels, at.lane, wide, full, 0);
+      request_rows += tile_steps;
     }
     commit_copies();
   };
   auto front_of = [&](int k) {
-    const int tile = (rounds - 1 - k) * split + at.rank;
-    return at.live && k < rounds && tile < count ? load_f(g.kept + ((long long)at.b * count + tile) * a.channels + at.c, static_cast<V*>(nullptr)) : all<VEC>(0.f);
+    const int tile = tile0 + rounds - 1 - k;
+    return at.live && k < rounds ? load_f(g.kept + ((long long)at.b * count + tile) * a.channels + at.c, static_cast<V*>(nullptr)) : all<VEC>(0.f);
   };
 #pragma unroll
   for (int k = 0; k < R::SLOTS - 1; ++k) request(k);
   const long long state_at = (long long)at.b * a.channels + at.c;
   // f_{t+1} dh_{t+1} at the end of what is left
   V carry = at.live && g.dlast != nullptr ? load_f(g.dlast + state_at, static_cast<V*>(nullptr)) : all<VEC>(0.f);
+  if (at.live)
+#pragma unroll 4
+    for (int z = ch.count * ch.pieces - 1; z >= (at.chunk + 1) * ch.pieces; --z) carry = after<CUT>(ch.run<VEC>(a, z, state_at), carry);
   V next_front = front_of(0);
   const Gate<T, VEC> forget(a.forget_bias), input(0.f);
   uint32_t cuts = 0, next_cuts = 0;
   if (CUT) next_cuts = load_cuts<STEPS>(a, at.b, t0_of(0), at.lane);
-  if (split > 1) tc::cluster_sync_all();
 
   for (int k = 0; k < rounds; ++k) {
     const int t0 = t0_of(k), buf = k & 1;
@@ -409,10 +512,12 @@ scan_bwd_kernel(const ScanArgs a, const ScanGrads g, const int wide, const int w
       if (k + 1 < rounds) next_cuts = load_cuts<STEPS>(a, at.b, t0_of(k + 1), at.lane);
     }
     const typename L::Raw* raw = reinterpret_cast<const typename L::Raw*>(ring + k % R::SLOTS * R::SLOT) + at.lane;
+    // read again where they are needed again: registers are what limits this kernel
     auto x_of = [&](int i) { return L::unpack(raw[(STEPS + i) * 32]); };
     auto dy_of = [&](int i) { return L::unpack(raw[(2 * STEPS + i) * 32]); };
     V f[STEPS], n[STEPS], u[GATE ? STEPS : 1], m[GATE ? STEPS : 1];              // sigmoids and their complements
     Run<VEC> sum = {all<VEC>(1.f), all<VEC>(0.f)};
+    V up = all<VEC>(0.f);                      // f_0 (dy_0 + f_1 (dy_1 + ...)), summed from the front
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
       forget(L::unpack(raw[i * 32]), f[i], n[i]);
@@ -421,58 +526,24 @@ scan_bwd_kernel(const ScanArgs a, const ScanGrads g, const int wide, const int w
       if (i == 0) sum = {f[0], w};
       else sum = {mul(sum.a, f[i]), fma(f[i], sum.b, w)};
       if (CUT && (cuts >> i & 1)) sum = {all<VEC>(-0.f), w};
+      const V more = fma(sum.a, dy_of(i), up);
+      up = CUT ? where_cut(sum.a, up, more) : more;
     }
-    V up = all<VEC>(0.f);
-#pragma unroll
-    for (int i = STEPS - 1; i >= 0; --i) {
-      up = mul(f[i], add(dy_of(i), up));
-      if (CUT && (cuts >> i & 1)) up = all<VEC>(0.f);
-    }
+    V end = carry;
     if (warps > 1) {
       parts[buf][at.warp][at.lane] = sum;
       back[buf][at.warp][at.lane] = up;
       __syncthreads();
-    }
-    V d = carry;
-    if (split > 1) {
-      Run<VEC> whole = {parts[buf][kWarps - 1][at.lane].a, back[buf][kWarps - 1][at.lane]};
-#pragma unroll
-      for (int j = kWarps - 2; j >= 0; --j) whole = joined<CUT>(whole, Run<VEC>{parts[buf][j][at.lane].a, back[buf][j][at.lane]});
-      for (int r = at.warp; r < split; r += kWarps) store_cluster(tc::map_to_cta(tc::smem_u32(&tiles[buf][at.rank][at.lane]), (uint32_t)r), whole);
-      __syncwarp();
-      tc::cluster_sync_all();
-      V behind = d;
+      if (k > 0) end = carries[buf ^ 1][at.first][at.lane];
 #pragma unroll 4
-      for (int r = split - 1; r >= 0; --r) {
-        if (r == at.rank) behind = d;
-        d = after<CUT>(tiles[buf][r][at.lane], d);
-      }
-      carry = d;
-      d = behind;
-    }
-    V end = d;
-    if (warps == kWarps) {
-      V h = start;
-#pragma unroll
-      for (int j = 0; j < kWarps; ++j) {
-        if (j == at.part) start = h;
-        if (j + 1 < kWarps) h = after<CUT>(parts[buf][j][at.lane], h);
-      }
-#pragma unroll
-      for (int j = kWarps - 1; j >= 0; --j) {
-        if (j == at.part) end = d;
-        d = after<CUT>(Run<VEC>{parts[buf][j][at.lane].a, back[buf][j][at.lane]}, d);
-      }
-    } else if (warps > 1) {
       for (int j = 0; j < at.part; ++j) start = after<CUT>(parts[buf][at.first + j][at.lane], start);
-      for (int j = warps - 1; j >= 0; --j) {
-        if (j == at.part) end = d;
-        d = after<CUT>(Run<VEC>{parts[buf][at.first + j][at.lane].a, back[buf][at.first + j][at.lane]}, d);
-      }
+#pragma unroll 4
+      for (int j = warps - 1; j > at.part; --j) end = after<CUT>(Run<VEC>{parts[buf][at.first + j][at.lane].a, back[buf][at.first + j][at.lane]}, end);
+      carry = after<CUT>(Run<VEC>{sum.a, up}, end);        // the first warp knows what the tile in front of this one ends on
+      if (at.part == 0) carries[buf][at.first][at.lane] = carry;
     } else {
-      d = after<CUT>(Run<VEC>{sum.a, up}, d);
+      carry = after<CUT>(Run<VEC>{sum.a, up}, end);
     }
-    if (split == 1) carry = d;
     // the states in front of each step, then dh from the last step to the first
     V before[STEPS];
 #pragma unroll
@@ -482,105 +553,116 @@ scan_bwd_kernel(const ScanArgs a, const ScanGrads g, const int wide, const int w
       start = fma(f[i], before[i], mul(GATE ? u[GATE ? i : 0] : n[i], x_of(i)));
     }
     const int rows = at.live ? a.steps - t0 : 0;
-    const long long out = ((long long)at.b * a.steps + t0 + STEPS - 1) * a.channels + at.c;
+    const long long out = ((long long)at.b * a.steps + t0) * a.channels + at.c;
     T *to_x = static_cast<T*>(g.dx) + out, *to_f = static_cast<T*>(g.dforget) + out, *to_i = static_cast<T*>(g.dinput) + (GATE ? out : 0);
+    const uint32_t row = (uint32_t)a.channels * (uint32_t)sizeof(T);
+    auto walk = [&](auto whole) {
 #pragma unroll
-    for (int i = STEPS - 1; i >= 0; --i) {
-      const V x = x_of(i), dh = add(end, dy_of(i));
-      const V dx = mul(dh, GATE ? u[GATE ? i : 0] : n[i]);
-      const V df = mul(mul(dh, GATE ? before[i] : fma(x, all<VEC>(-1.f), before[i])), mul(f[i], n[i]));
-      end = mul(f[i], dh);
-      if (CUT && (cuts >> i & 1)) end = all<VEC>(0.f);
-      if (i < rows) {
-        L::store(to_x, dx);
-        L::store(to_f, df);
-        if constexpr (GATE) L::store(to_i, mul(mul(dh, x), mul(u[i], m[i])));
+      for (int i = STEPS - 1; i >= 0; --i) {
+        const V x = x_of(i), dh = add(end, dy_of(i));
+        const V dx = mul(dh, GATE ? u[GATE ? i : 0] : n[i]);
+        const V df = mul(mul(dh, GATE ? before[i] : fma(x, all<VEC>(-1.f), before[i])), mul(f[i], n[i]));
+        end = mul(f[i], dh);
+        if (CUT && (cuts >> i & 1)) end = all<VEC>(0.f);
+        if (whole.value || i < rows) {
+          L::store(row_at(to_x, row, i), dx);
+          L::store(row_at(to_f, row, i), df);
+          if constexpr (GATE) L::store(row_at(to_i, row, i), mul(mul(dh, x), mul(u[i], m[i])));
+        }
       }
-      to_x -= a.channels;
-      to_f -= a.channels;
-      if constexpr (GATE) to_i -= a.channels;
-    }
+    };
+    if (rows >= STEPS) walk(std::true_type());
+    else walk(std::false_type());
     __syncwarp();                              // the slot has been read
   }
   wait_copies<0>();
-  if (at.rank == 0 && at.part == 0 && at.live) store_f(g.dstate + state_at, carry);
+  if (at.chunk == 0 && at.part == 0 && at.live) store_f(g.dstate + state_at, carry);
 }
 
 // How a call is laid out: a warp alone on its channels where that makes kBusy warps for every SM; else more warps side by side in time; else
-// clusters. The backward pass's part of this decides what the forward pass keeps, so it goes by sizes alone.
+// chunks. The backward pass's part of the warps decides what the forward pass keeps, so it goes by sizes alone.
 constexpr long long kBusy = 16;
-struct Shape { int warps, split, threads; unsigned blocks; };
+constexpr int kResident = 2;                 // blocks on an SM
+constexpr int kPieceBlocks = 3;              // of the kernel that goes ahead
 int warps_of(const ScanArgs& a, int steps) {
   const long long columns = (long long)a.batch * ((a.channels + 63) / 64), runs = (a.steps + steps - 1) / steps;
   int warps = 1;
   while (warps < kWarps && warps < runs && columns * warps < kBusy * sm_count()) warps *= 2;
   return warps;
 }
-Shape shape_of(const ScanArgs& a, int vec, int steps) {
-  const long long columns = (long long)a.batch * ((a.channels + 32 * vec - 1) / (32 * vec));
-  Shape s;
-  s.warps = warps_of(a, steps);
-  const int beside = kWarps / s.warps;
-  s.threads = 32 * kWarps;
-  s.split = 1;
-  const long long tiles = (a.steps + s.warps * steps - 1) / (s.warps * steps);
-  if (s.warps == kWarps)
-    while (s.split < kMostSplit && tiles >= 2 * s.split && columns * s.split * kWarps < kBusy * sm_count()) s.split *= 2;
-  s.blocks = (unsigned)((columns + beside - 1) / beside * s.split);
-  return s;
+long long columns_of(const ScanArgs& a, int vec) { return (long long)a.batch * ((a.channels + 32 * vec - 1) / (32 * vec)); }
+// As many chunks as make one block for every place on the SMs, and as many pieces of them for the kernel that goes ahead.
+Chunks chunks_of(const ScanArgs& a, int vec, int warps, int steps, float* runs) {
+  const long long columns = columns_of(a, vec);
+  const int tiles = (a.steps + warps * steps - 1) / (warps * steps);
+  long long count = warps == kWarps && runs != nullptr ? kResident * sm_count() / columns : 1;
+  if (count > tiles / kLeastTiles) count = tiles / kLeastTiles;
+  if (count < 2) return {1, tiles, 1, nullptr};
+  const int each = (int)((tiles + count - 1) / count);
+  count = (tiles + each - 1) / each;
+  long long pieces = kPieceBlocks * sm_count() / (columns * (count - 1));
+  if (pieces > 32 / (count - 1)) pieces = 32 / (count - 1);              // a block folds them one after the other
+  return {(int)count, each, (int)(pieces < 1 ? 1 : pieces > each ? each : pieces), runs};
 }
 
-template <typename... K, typename... A>
-cudaError_t launch(void (*kernel)(K...), const Shape& s, size_t smem, cudaStream_t st, const A&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(s.blocks);
-  cfg.blockDim = dim3(s.threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = (unsigned)s.split; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr; cfg.numAttrs = s.split > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args..., s.warps, s.split);
-}
-// More shared memory than a kernel has by itself, and clusters of more than 8 blocks, have to be asked for, once per kernel.
+// More shared memory than a kernel has by itself has to be asked for, once per kernel.
 template <class Kernel>
-cudaError_t allow(Kernel kernel, size_t smem) {
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  return e != cudaSuccess ? e : cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+cudaError_t allow(Kernel kernel, size_t smem) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); }
+
+int tile_log2(const ScanArgs& a) {
+  int log2 = 0;
+  while (1 << log2 < warps_of(a, kBack) * kBack) ++log2;
+  return log2;
 }
 
-int tile_of(const ScanArgs& a) { return warps_of(a, kBack) * kBack; }
-
+template <typename T, int VEC, bool GATE, bool CUT, bool BACK>
+cudaError_t run_chunks(const ScanArgs& a, const ScanView& dy, int wide, int tile_steps, const Chunks& ch, cudaStream_t st) {
+  if (ch.count == 1) return cudaSuccess;
+  auto kernel = scan_chunks_kernel<T, VEC, GATE, CUT, BACK>;
+  constexpr size_t smem = kWarps * Ring<T, VEC, kBack, GATE && !BACK ? 3 : 2>::BYTES;
+  static const cudaError_t allowed = allow(kernel, smem);
+  if (allowed != cudaSuccess) return allowed;
+  return launch_pdl(kernel, dim3((unsigned)(columns_of(a, VEC) * (ch.count - 1) * ch.pieces)), dim3(32 * kWarps), smem, st, a, dy, wide, tile_steps, ch);
+}
 template <typename T, int VEC, bool GATE, bool CUT, int STEPS>
-cudaError_t run_forward(const ScanArgs& a, void* y, float* last, float* kept, int wide, cudaStream_t st) {
+cudaError_t run_forward(const ScanArgs& a, void* y, float* last, float* kept, float* runs, int wide, int* launched, cudaStream_t st) {
   auto kernel = scan_fwd_kernel<T, VEC, GATE, CUT, STEPS>;
   constexpr size_t smem = kWarps * Ring<T, VEC, STEPS, GATE ? 3 : 2>::BYTES;
   static const cudaError_t allowed = allow(kernel, smem);
   if (allowed != cudaSuccess) return allowed;
-  const Shape s = shape_of(a, VEC, STEPS);
-  return launch(kernel, s, smem, st, a, static_cast<T*>(y), last, kept, tile_of(a), wide);
+  const int warps = warps_of(a, STEPS), beside = kWarps / warps;
+  const Chunks ch = chunks_of(a, VEC, warps, STEPS, runs);
+  const cudaError_t e = run_chunks<T, VEC, GATE, CUT, false>(a, a.x, wide, warps * STEPS, ch, st);
+  if (e != cudaSuccess) return e;
+  *launched = ch.count > 1 ? 2 : 1;
+  const unsigned blocks = (unsigned)((columns_of(a, VEC) + beside - 1) / beside * ch.count);
+  return launch_pdl(kernel, dim3(blocks), dim3(32 * kWarps), smem, st, a, static_cast<T*>(y), last, kept, tile_log2(a), wide, warps, ch);
 }
 template <typename T, int VEC, bool GATE, bool CUT>
-cudaError_t run_backward(const ScanArgs& a, const ScanGrads& g, int wide, cudaStream_t st) {
+cudaError_t run_backward(const ScanArgs& a, const ScanGrads& g, float* runs, int wide, int* launched, cudaStream_t st) {
   auto kernel = scan_bwd_kernel<T, VEC, GATE, CUT>;
   constexpr size_t smem = kWarps * Ring<T, VEC, kBack, GATE ? 4 : 3>::BYTES;
   static const cudaError_t allowed = allow(kernel, smem);
   if (allowed != cudaSuccess) return allowed;
-  return launch(kernel, shape_of(a, VEC, kBack), smem, st, a, g, wide);
+  const int warps = warps_of(a, kBack), beside = kWarps / warps;
+  const Chunks ch = chunks_of(a, VEC, warps, kBack, runs);
+  const cudaError_t e = run_chunks<T, VEC, GATE, CUT, true>(a, g.dy, wide, warps * kBack, ch, st);
+  if (e != cudaSuccess) return e;
+  *launched = ch.count > 1 ? 2 : 1;
+  const unsigned blocks = (unsigned)((columns_of(a, VEC) + beside - 1) / beside * ch.count);
+  return launch_pdl(kernel, dim3(blocks), dim3(32 * kWarps), smem, st, a, g, wide, warps, ch);
 }
+
 template <typename T, int VEC, int STEPS>
-cudaError_t forward(const ScanArgs& a, void* y, float* last, float* kept, int wide, cudaStream_t st) {
+cudaError_t forward(const ScanArgs& a, void* y, float* last, float* kept, float* runs, int wide, int* launched, cudaStream_t st) {
   if (a.reset != nullptr)
-    return a.input.p != nullptr ? run_forward<T, VEC, true, true, STEPS>(a, y, last, kept, wide, st) : run_forward<T, VEC, false, true, STEPS>(a, y, last, kept, wide, st);
-  return a.input.p != nullptr ? run_forward<T, VEC, true, false, STEPS>(a, y, last, kept, wide, st) : run_forward<T, VEC, false, false, STEPS>(a, y, last, kept, wide, st);
+    return a.input.p != nullptr ? run_forward<T, VEC, true, true, STEPS>(a, y, last, kept, runs, wide, launched, st) : run_forward<T, VEC, false, true, STEPS>(a, y, last, kept, runs, wide, launched, st);
+  return a.input.p != nullptr ? run_forward<T, VEC, true, false, STEPS>(a, y, last, kept, runs, wide, launched, st) : run_forward<T, VEC, false, false, STEPS>(a, y, last, kept, runs, wide, launched, st);
 }
 template <typename T, int VEC>
-cudaError_t backward(const ScanArgs& a, const ScanGrads& g, int wide, cudaStream_t st) {
-  if (a.reset != nullptr) return a.input.p != nullptr ? run_backward<T, VEC, true, true>(a, g, wide, st) : run_backward<T, VEC, false, true>(a, g, wide, st);
-  return a.input.p != nullptr ? run_backward<T, VEC, true, false>(a, g, wide, st) : run_backward<T, VEC, false, false>(a, g, wide, st);
+cudaError_t backward(const ScanArgs& a, const ScanGrads& g, float* runs, int wide, int* launched, cudaStream_t st) {
+  if (a.reset != nullptr) return a.input.p != nullptr ? run_backward<T, VEC, true, true>(a, g, runs, wide, launched, st) : run_backward<T, VEC, false, true>(a, g, runs, wide, launched, st);
+  return a.input.p != nullptr ? run_backward<T, VEC, true, false>(a, g, runs, wide, launched, st) : run_backward<T, VEC, false, false>(a, g, runs, wide, launched, st);
 }
 
 // Whether all views' rows start on multiples of `bytes` and hold whole pieces of as many.
@@ -599,22 +681,34 @@ bool floats_in_pairs(std::initializer_list<const float*> vectors) {
 
 }  // namespace
 
-int gated_scan_tile(const ScanArgs& a) { return tile_of(a); }
-
-cudaError_t gated_scan_fwd(const ScanArgs& a, void* y, float* last, float* kept, cudaStream_t st) {
-  if (a.batch <= 0 || a.channels <= 0) return cudaSuccess;
-  const bool pairs = rows_fit(a, a.bf16 ? 4 : 8, {a.x, a.forget, a.input}) && floats_in_pairs({a.state, last, kept});
-  const int wide = rows_fit(a, 16, {a.x, a.forget, a.input});
-  if (!a.bf16) return pairs ? forward<float, 2, 8>(a, y, last, kept, wide, st) : forward<float, 1, 8>(a, y, last, kept, wide, st);
-  if (!pairs) return forward<bf16, 1, 8>(a, y, last, kept, wide, st);
-  return a.input.p == nullptr && a.steps >= 16 * kWarps ? forward<bf16, 2, 16>(a, y, last, kept, wide, st) : forward<bf16, 2, 8>(a, y, last, kept, wide, st);
+long long gated_scan_runs(const ScanArgs& a) {
+  if (warps_of(a, kBack) < kWarps) return 0;
+  // columns * (count - 1) * pieces is at most kPieceBlocks * SMs, or pieces is 1 and columns * count at most kResident * SMs
+  const long long columns = columns_of(a, 2), most = (kPieceBlocks + kResident) * sm_count() / columns;
+  return kResident * sm_count() / columns < 2 || a.steps < 2 * kLeastTiles * kWarps * kBack ? 0 : 2 * 2 * most * a.batch * a.channels;
 }
-cudaError_t gated_scan_bwd(const ScanArgs& a, const ScanGrads& g, cudaStream_t st) {
+int gated_scan_tile(const ScanArgs& a) { return 1 << tile_log2(a); }
+
+cudaError_t gated_scan_fwd(const ScanArgs& a, void* y, float* last, float* kept, float* runs, int* launched, cudaStream_t st) {
+  *launched = 0;
   if (a.batch <= 0 || a.channels <= 0) return cudaSuccess;
-  const bool pairs = rows_fit(a, a.bf16 ? 4 : 8, {a.x, a.forget, a.input, g.dy}) && floats_in_pairs({g.kept, g.dlast, g.dstate});
+  const bool pairs = rows_fit(a, a.bf16 ? 4 : 8, {a.x, a.forget, a.input}) && floats_in_pairs({a.state, last, kept, runs});
+  const int wide = rows_fit(a, 16, {a.x, a.forget, a.input});
+  const bool longer = a.steps >= 16 * kWarps;
+  if (!a.bf16) {
+    if (pairs) return forward<float, 2, 8>(a, y, last, kept, runs, wide, launched, st);
+    return longer ? forward<float, 1, 16>(a, y, last, kept, runs, wide, launched, st) : forward<float, 1, 8>(a, y, last, kept, runs, wide, launched, st);
+  }
+  if (pairs) return longer && a.input.p == nullptr ? forward<bf16, 2, 16>(a, y, last, kept, runs, wide, launched, st) : forward<bf16, 2, 8>(a, y, last, kept, runs, wide, launched, st);
+  return longer ? forward<bf16, 1, 16>(a, y, last, kept, runs, wide, launched, st) : forward<bf16, 1, 8>(a, y, last, kept, runs, wide, launched, st);
+}
+cudaError_t gated_scan_bwd(const ScanArgs& a, const ScanGrads& g, float* runs, int* launched, cudaStream_t st) {
+  *launched = 0;
+  if (a.batch <= 0 || a.channels <= 0) return cudaSuccess;
+  const bool pairs = rows_fit(a, a.bf16 ? 4 : 8, {a.x, a.forget, a.input, g.dy}) && floats_in_pairs({g.kept, g.dlast, g.dstate, runs});
   const int wide = rows_fit(a, 16, {a.x, a.forget, a.input, g.dy});
-  if (!a.bf16) return pairs ? backward<float, 2>(a, g, wide, st) : backward<float, 1>(a, g, wide, st);
-  return pairs ? backward<bf16, 2>(a, g, wide, st) : backward<bf16, 1>(a, g, wide, st);
+  if (!a.bf16) return pairs ? backward<float, 2>(a, g, runs, wide, launched, st) : backward<float, 1>(a, g, runs, wide, launched, st);
+  return pairs ? backward<bf16, 2>(a, g, runs, wide, launched, st) : backward<bf16, 1>(a, g, runs, wide, launched, st);
 }
 
 }  // namespace adb200

@@ -19,7 +19,9 @@ struct ScanArgs {
 int gated_scan_tile(const ScanArgs& a);
 // y: [batch, steps, channels], last: [batch, channels]; kept (nullptr: not wanted): [batch, ceil(steps / gated_scan_tile), channels], the states
 // in front of each tile
-cudaError_t gated_scan_fwd(const ScanArgs& a, void* y, float* last, float* kept, cudaStream_t st);
+// runs: gated_scan_runs(a) floats of scratch, for either pass; launched: how many kernels it took
+long long gated_scan_runs(const ScanArgs& a);
+cudaError_t gated_scan_fwd(const ScanArgs& a, void* y, float* last, float* kept, float* runs, int* launched, cudaStream_t st);
 
 struct ScanGrads {
   ScanView dy;                             // p == nullptr: zeros
@@ -28,6 +30,6 @@ struct ScanGrads {
   void *dx, *dforget, *dinput;             // [batch, steps, channels]; dinput only with an input gate
   float* dstate;                           // [batch, channels]
 };
-cudaError_t gated_scan_bwd(const ScanArgs& a, const ScanGrads& g, cudaStream_t st);
+cudaError_t gated_scan_bwd(const ScanArgs& a, const ScanGrads& g, float* runs, int* launched, cudaStream_t st);
 
 }  // namespace adb200

@@ -49,7 +49,8 @@ class _Counting:
               "sampled_logits": 2, "sampled_grad": 2, "sampled_bias_grad": 2, "conv_dgrad": _dgrad_launches, "rms_norm_bwd": 3}
 
     #: kernels per call where that depends on what the call returned
-    _AFTER = {"copy_list": _copy_list_launches, "adamw_list_step": lambda launched, *args: launched}
+    _AFTER = {"copy_list": _copy_list_launches, "adamw_list_step": lambda launched, *args: launched,
+              "gated_scan_fwd": lambda result, *args: result[-1], "gated_scan_bwd": lambda result, *args: result[-1]}
 
     def __init__(self, mod):
         self._mod = mod

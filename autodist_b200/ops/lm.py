@@ -168,7 +168,7 @@ def _scan_plain(x, forget, input_gate, state, reset, forget_bias):
 class _GatedRecurrenceFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, forget, input_gate, state, reset, forget_bias):
-        y, last, kept = ops.ext(required=True).gated_scan_fwd(x, forget, input_gate, state, reset, forget_bias, True)
+        y, last, kept, _ = ops.ext(required=True).gated_scan_fwd(x, forget, input_gate, state, reset, forget_bias, True)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, forget, input_gate, state, reset, kept)
         ctx.forget_bias = forget_bias
@@ -212,5 +212,5 @@ def gated_recurrence(x, forget, input_gate=None, state=None, reset=None, forget_
         return _scan_plain(x, forget, input_gate, state, reset, forget_bias)
     if _wants_gradient(x, forget, input_gate, state):
         return _GatedRecurrenceFn.apply(x, forget, input_gate, state, reset, float(forget_bias))
-    y, last, _ = ops.ext(required=True).gated_scan_fwd(x, forget, input_gate, state, reset, forget_bias, False)
+    y, last, _, _ = ops.ext(required=True).gated_scan_fwd(x, forget, input_gate, state, reset, forget_bias, False)
     return y, last
