@@ -4,8 +4,10 @@
 #include <cuda_runtime.h>
 #include <torch/extension.h>
 
+#include <atomic>
 #include <memory>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "adamw_list.h"
@@ -67,6 +69,24 @@ Tensor check_weight(const Tensor& x, const Tensor& weight, const char* name) {
   TORCH_CHECK(weight.scalar_type() == at::kFloat || weight.scalar_type() == x.scalar_type(), name, ": the weight must be fp32 or of the input's type, got ", shown(weight));
   return weight.contiguous();
 }
+
+// ---------------------------------------------------------------------------------------------- gradients
+// Kernels that backward passes launched: those run in the autograd engine, not through the counted calls.
+constexpr int kNormBackwardKernels = 3;
+std::atomic<int64_t> g_backward_kernels{0};
+int64_t backward_kernels() { return g_backward_kernels.load(); }
+
+// Gradients that can be differentiated themselves: the same expression in PyTorch operations, by `name` in autodist_b200.ops.lm.
+template <typename... Args>
+torch::autograd::variable_list differentiable(const char* name, size_t inputs, Args&&... args) {
+  pybind11::gil_scoped_acquire gil;
+  const auto found = pybind11::module_::import("autodist_b200.ops.lm").attr(name)(std::forward<Args>(args)...).template cast<std::vector<optional<Tensor>>>();
+  torch::autograd::variable_list grads;
+  for (const auto& g : found) grads.push_back(g.has_value() ? *g : Tensor());
+  grads.resize(inputs);
+  return grads;
+}
+optional<Tensor> some(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : c10::nullopt; }
 
 struct NormInputs {                        // what the addresses in `rows` belong to
   Tensor x, res, weight, sum;
@@ -133,6 +153,37 @@ std::tuple<Tensor, Tensor> rms_norm_bwd(const Tensor& dy, const optional<Tensor>
   g.dx = dx.data_ptr(); g.dw = dw.data_ptr(); g.part = part.data_ptr<float>();
   launched(adb200::rms_norm_bwd(g, stream_of(s)), name);
   return {dx, dw};
+}
+
+class NormFunction : public torch::autograd::Function<NormFunction> {
+ public:
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& weight, const optional<Tensor>& residual, double eps) {
+    auto [y, sum] = rms_norm_fwd(x, weight, residual, eps);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({sum.has_value() ? *sum : x, weight});
+    ctx->saved_data["eps"] = eps;
+    return sum.has_value() ? torch::autograd::variable_list{y, *sum} : torch::autograd::variable_list{y};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const bool residual = grads.size() > 1;
+    const Tensor ds = residual ? grads[1] : Tensor();
+    const double eps = ctx->saved_data["eps"].toDouble();
+    // the sum is the only place where x and the residual meet: both get its gradient
+    if (!grads[0].defined()) return {ds, Tensor(), ds, Tensor()};
+    if (at::GradMode::is_enabled()) {
+      auto again = differentiable("_norm_again", 2, saved[0], saved[1], eps, grads[0], some(ds));
+      return {again[0], again[1], residual ? again[0] : Tensor(), Tensor()};
+    }
+    auto [dx, dw] = rms_norm_bwd(grads[0], some(ds), saved[0], saved[1], eps);
+    g_backward_kernels += kNormBackwardKernels;
+    return {dx, dw, residual ? dx : Tensor(), Tensor()};
+  }
+};
+// -> (y, x + residual), with a gradient where one is recorded
+std::tuple<Tensor, optional<Tensor>> rms_norm(const Tensor& x, const Tensor& weight, const optional<Tensor>& residual, double eps) {
+  const auto out = NormFunction::apply(x, weight, residual, eps);
+  return {out[0], out.size() > 1 ? optional<Tensor>(out[1]) : c10::nullopt};
 }
 
 // Codes of [..., width] whose rows start on 16-byte boundaries.
@@ -307,6 +358,47 @@ std::tuple<Tensor, Tensor, optional<Tensor>, Tensor, int> gated_scan_bwd(const o
   return {dx, dforget, input.has_value() ? optional<Tensor>(dinput) : c10::nullopt, dstate, kernels};
 }
 
+class ScanFunction : public torch::autograd::Function<ScanFunction> {
+ public:
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& forget, const optional<Tensor>& input,
+                                                const optional<Tensor>& state, const optional<Tensor>& reset, double forget_bias, bool keep, int* kernels) {
+    auto [y, last, kept, launches] = gated_scan_fwd(x, forget, input, state, reset, forget_bias, keep);
+    *kernels = launches;
+    if (keep) {
+      ctx->set_materialize_grads(false);
+      ctx->save_for_backward({x, forget, input.value_or(Tensor()), state.value_or(Tensor()), reset.value_or(Tensor()), *kept});
+      ctx->saved_data["forget_bias"] = forget_bias;
+    }
+    return {y, last};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const double forget_bias = ctx->saved_data["forget_bias"].toDouble();
+    torch::autograd::variable_list found;
+    if (!grads[0].defined() && !grads[1].defined()) {
+      found.resize(4);
+    } else if (at::GradMode::is_enabled()) {
+      found = differentiable("_scan_again", 4, saved[0], saved[1], some(saved[2]), some(saved[3]), some(saved[4]), forget_bias, some(grads[0]), some(grads[1]));
+    } else {
+      auto [dx, dforget, dinput, dstate, launches] = gated_scan_bwd(some(grads[0]), some(grads[1]), saved[0], saved[1], some(saved[2]), some(saved[3]), some(saved[4]),
+                                                                    saved[5], forget_bias);
+      g_backward_kernels += launches;
+      found = {dx, dforget, dinput.value_or(Tensor()), saved[3].defined() ? dstate : Tensor()};
+    }
+    found.resize(8);
+    return found;
+  }
+};
+// -> (outputs, last state, kernels launched), with a gradient where one is recorded
+std::tuple<Tensor, Tensor, int> gated_scan(const Tensor& x, const Tensor& forget, const optional<Tensor>& input, const optional<Tensor>& state,
+                                           const optional<Tensor>& reset, double forget_bias) {
+  const bool keep = at::GradMode::is_enabled() && (x.requires_grad() || forget.requires_grad() || (input.has_value() && input->requires_grad()) ||
+                                                   (state.has_value() && state->requires_grad()));
+  int kernels = 0;
+  const auto out = ScanFunction::apply(x, forget, input, state, reset, forget_bias, keep, &kernels);
+  return {out[0], out[1], kernels};
+}
+
 // ---------------------------------------------------------------------------------------------- optimizer
 // The parameters of a group and where their moments lie. Addresses are read at every step: a parameter's storage may change.
 struct AdamwList {
@@ -399,6 +491,10 @@ int64_t adamw_list_step(const std::shared_ptr<AdamwList>& l, double lr, const op
 }  // namespace
 
 void register_lm(pybind11::module& m) {
+  m.def("rms_norm", &rms_norm);
+  m.def("gated_scan", &gated_scan);
+  m.def("backward_kernels", &backward_kernels);
+  m.attr("NORM_BACKWARD_KERNELS") = kNormBackwardKernels;
   m.def("rms_norm_fwd", &rms_norm_fwd);
   m.def("rms_norm_bwd", &rms_norm_bwd);
   m.def("rms_norm_8bit", &rms_norm_8bit);

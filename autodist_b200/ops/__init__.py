@@ -7,6 +7,7 @@ device ``ext()`` returns ``None`` and only the host-side logic is usable.
 import importlib.util
 import os
 import sys
+import types
 
 import torch
 
@@ -14,7 +15,18 @@ from autodist_b200.ops import build as _build
 
 _EXT = None
 _TRIED = False
-launch_count = 0      # kernels launched through the extension by this process (a graph replay re-launches its capture)
+_counted = 0
+
+
+class _Ops(types.ModuleType):
+    @property
+    def launch_count(self):
+        """Kernels launched through the extension by this process, backward passes in the autograd engine among them (a graph replay
+        re-launches its capture)."""
+        return _counted + (0 if _EXT is None else _EXT.backward_kernels())
+
+
+sys.modules[__name__].__class__ = _Ops
 
 
 def _dgrad_launches(dy, w, dx, stride, pad, *_):
@@ -40,7 +52,7 @@ def _copy_list_launches(taken, dst, src):
 class _Counting:
     """Thin proxy over the extension module that counts kernel-launching calls."""
     _NO_LAUNCH = {"ln_bwd_part_floats", "sampled_grad_chunks", "sampled_bias_chunks", "bce_logits_parts", "colsum_parts", "gemm_choice", "gemm_set_trace", "conv_set_trace", "MAX_COMM_BLOCKS",
-                  "adamw_list"}
+                  "adamw_list", "backward_kernels", "NORM_BACKWARD_KERNELS"}
     #: kernels per call where that is not one: a number, or a function of the call's arguments
     _MULTI = {"ln_bwd": 2, "keyed_colsum": 2, "relu_bwd_colsum": 2, "bn_sums": 2, "bn_bwd": 2,
               "bn_fwd": lambda *a: 1 if a[9] is not None else 3, "bn_fwd_nchw": lambda *a: 1 if a[6] is not None else 3,       # sums given or not
@@ -50,7 +62,8 @@ class _Counting:
 
     #: kernels per call where that depends on what the call returned
     _AFTER = {"copy_list": _copy_list_launches, "adamw_list_step": lambda launched, *args: launched,
-              "gated_scan_fwd": lambda result, *args: result[-1], "gated_scan_bwd": lambda result, *args: result[-1]}
+              "gated_scan_fwd": lambda result, *args: result[-1], "gated_scan_bwd": lambda result, *args: result[-1],
+              "gated_scan": lambda result, *args: result[-1]}
 
     def __init__(self, mod):
         self._mod = mod
@@ -66,9 +79,9 @@ class _Counting:
     @staticmethod
     def _wrap_after(fn, launches):
         def call(*args):
-            global launch_count
+            global _counted
             result = fn(*args)
-            launch_count += launches(result, *args)
+            _counted += launches(result, *args)
             return result
         return call
 
@@ -76,13 +89,13 @@ class _Counting:
     def _wrap(fn, n):
         if callable(n):
             def call(*args):
-                global launch_count
-                launch_count += n(*args)
+                global _counted
+                _counted += n(*args)
                 return fn(*args)
         else:
             def call(*args):
-                global launch_count
-                launch_count += n
+                global _counted
+                _counted += n
                 return fn(*args)
         return call
 

@@ -26,12 +26,14 @@ def _wants_gradient(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
-def _differentiated_again(plain, inputs, needed, grads_of_outputs):
-    """Gradients of ``plain(*inputs)`` that can be differentiated themselves (``create_graph``), ``None`` where none is needed."""
-    wanted = [t for t, w in zip(inputs, needed) if w]
+def _differentiated_again(plain, inputs, grads_of_outputs):
+    """Gradients of ``plain(*inputs)`` that can be differentiated themselves (``create_graph``); ``None`` for inputs that need none."""
+    wanted = [t is not None and t.requires_grad for t in inputs]
+    # aliases: what is being differentiated may be an output of the very node that asks, which the engine has locked
+    inputs = [t.view_as(t) if w else t for t, w in zip(inputs, wanted)]
     outs, grads = zip(*((o, g) for o, g in zip(plain(*inputs), grads_of_outputs) if g is not None))
-    found = iter(torch.autograd.grad(outs, wanted, grads, create_graph=True, allow_unused=True))
-    return [next(found) if w else None for w in needed]
+    found = iter(torch.autograd.grad(outs, [t for t, w in zip(inputs, wanted) if w], grads, create_graph=True, allow_unused=True))
+    return [next(found) if w else None for w in wanted]
 
 
 # ---------------------------------------------------------------------------------------------------------------- norm
@@ -55,28 +57,9 @@ def _norm_plain(x, weight, residual, eps):
     return y, s
 
 
-class _RMSNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, residual, eps):
-        y, s = ops.ext(required=True).rms_norm_fwd(x, weight, residual, eps)
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x if residual is None else s, weight)
-        ctx.eps = eps
-        return (y, s) if residual is not None else y
-
-    @staticmethod
-    def backward(ctx, dy, ds=None):
-        s, weight = ctx.saved_tensors
-        need_x, need_w, need_r, _ = ctx.needs_input_grad
-        if dy is None:
-            return ds if need_x else None, None, ds if need_r else None, None
-        if torch.is_grad_enabled():
-            # the sum is the only place where x and the residual meet: both get its gradient
-            dx, dw = _differentiated_again(lambda t, w: (_norm_plain(t, w, None, ctx.eps)[0].to(t.dtype), t), (s, weight),
-                                           (need_x or need_r, need_w), (dy, ds))
-        else:
-            dx, dw = ops.ext(required=True).rms_norm_bwd(dy, ds, s, weight, ctx.eps)
-        return dx if need_x else None, dw if need_w else None, dx if need_r else None, None
+def _norm_again(s, weight, eps, dy, ds):
+    """Gradients of what was normed and of the weight, for ``create_graph``."""
+    return _differentiated_again(lambda t, w: (_norm_plain(t, w, None, eps)[0].to(t.dtype), t), (s, weight), (dy, ds))
 
 
 def rms_norm(x, weight, residual=None, eps=1e-6):
@@ -86,9 +69,7 @@ def rms_norm(x, weight, residual=None, eps=1e-6):
     if not _kernels(x):
         y, s = _norm_plain(x, weight, residual, eps)
         return y.to(x.dtype) if residual is None else (y.to(x.dtype), s)
-    if _wants_gradient(x, weight, residual):
-        return _RMSNormFn.apply(x, weight, residual, eps)
-    y, s = ops.ext(required=True).rms_norm_fwd(x, weight, residual, eps)
+    y, s = ops.ext(required=True).rms_norm(x, weight, residual, eps)
     return y if residual is None else (y, s)
 
 
@@ -165,27 +146,9 @@ def _scan_plain(x, forget, input_gate, state, reset, forget_bias):
     return y, h if outs or state is None else h.clone()
 
 
-class _GatedRecurrenceFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, forget, input_gate, state, reset, forget_bias):
-        y, last, kept, _ = ops.ext(required=True).gated_scan_fwd(x, forget, input_gate, state, reset, forget_bias, True)
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x, forget, input_gate, state, reset, kept)
-        ctx.forget_bias = forget_bias
-        return y, last
-
-    @staticmethod
-    def backward(ctx, dy, dlast):
-        x, forget, input_gate, state, reset, kept = ctx.saved_tensors
-        needed = ctx.needs_input_grad[:4]
-        if dy is None and dlast is None:
-            return (None,) * 6
-        if torch.is_grad_enabled():
-            grads = _differentiated_again(lambda *a: _scan_plain(*a, reset, ctx.forget_bias), (x, forget, input_gate, state), needed, (dy, dlast))
-        else:
-            dlast = None if dlast is None else dlast.float()
-            grads = ops.ext(required=True).gated_scan_bwd(dy, dlast, x, forget, input_gate, state, reset, kept, ctx.forget_bias)
-        return tuple(g if w else None for g, w in zip(grads, needed)) + (None, None)
+def _scan_again(x, forget, input_gate, state, reset, forget_bias, dy, dlast):
+    """Gradients of the first four, for ``create_graph``."""
+    return _differentiated_again(lambda *a: _scan_plain(*a, reset, forget_bias), (x, forget, input_gate, state), (dy, dlast))
 
 
 def gated_recurrence(x, forget, input_gate=None, state=None, reset=None, forget_bias=0.0):
@@ -210,7 +173,5 @@ def gated_recurrence(x, forget, input_gate=None, state=None, reset=None, forget_
         raise ValueError(f"gated_recurrence: a finite forget_bias needed, got {forget_bias}")
     if not _kernels(x):
         return _scan_plain(x, forget, input_gate, state, reset, forget_bias)
-    if _wants_gradient(x, forget, input_gate, state):
-        return _GatedRecurrenceFn.apply(x, forget, input_gate, state, reset, float(forget_bias))
-    y, last, _, _ = ops.ext(required=True).gated_scan_fwd(x, forget, input_gate, state, reset, forget_bias, False)
+    y, last, _ = ops.ext(required=True).gated_scan(x, forget, input_gate, state, reset, forget_bias)
     return y, last
