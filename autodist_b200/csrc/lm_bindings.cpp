@@ -72,7 +72,6 @@ Tensor check_weight(const Tensor& x, const Tensor& weight, const char* name) {
 
 // ---------------------------------------------------------------------------------------------- gradients
 // Kernels that backward passes launched: those run in the autograd engine, not through the counted calls.
-constexpr int kNormBackwardKernels = 3;
 std::atomic<int64_t> g_backward_kernels{0};
 int64_t backward_kernels() { return g_backward_kernels.load(); }
 
@@ -128,8 +127,8 @@ std::tuple<Tensor, optional<Tensor>> rms_norm_fwd(const Tensor& x, const Tensor&
   return {y, residual.has_value() ? optional<Tensor>(in.sum) : c10::nullopt};
 }
 
-// -> (gradient of the input and of the residual, gradient of the weight)
-std::tuple<Tensor, Tensor> rms_norm_bwd(const Tensor& dy, const optional<Tensor>& ds, const Tensor& s, const Tensor& weight, double eps) {
+// -> (gradient of the input and of the residual, gradient of the weight, kernels launched)
+std::tuple<Tensor, Tensor, int> rms_norm_bwd(const Tensor& dy, const optional<Tensor>& ds, const Tensor& s, const Tensor& weight, double eps) {
   const char* name = "rms_norm";
   TORCH_CHECK(s.is_cuda(), "rms_norm: a tensor on a GPU needed");
   const c10::cuda::CUDAGuard guard(s.device());
@@ -149,10 +148,12 @@ std::tuple<Tensor, Tensor> rms_norm_bwd(const Tensor& dy, const optional<Tensor>
   g.weight = w.data_ptr(); g.weight_bf16 = w.scalar_type() == at::kBFloat16;
   g.rows = rows.size(0); g.width = (int)width; g.eps = (float)eps;
   Tensor dx = at::empty(s.sizes(), s.options()), dw = at::empty(w.sizes(), w.options());
-  Tensor part = at::empty({(int64_t)adb200::rms_norm_bwd_parts(g.rows, g.width) * width}, s.options().dtype(at::kFloat));
-  g.dx = dx.data_ptr(); g.dw = dw.data_ptr(); g.part = part.data_ptr<float>();
-  launched(adb200::rms_norm_bwd(g, stream_of(s)), name);
-  return {dx, dw};
+  g.dx = dx.data_ptr(); g.dw = dw.data_ptr();
+  Tensor part = at::empty({adb200::rms_norm_bwd_floats(g)}, s.options().dtype(at::kFloat));
+  g.part = part.data_ptr<float>();
+  int kernels = 0;
+  launched(adb200::rms_norm_bwd(g, &kernels, stream_of(s)), name);
+  return {dx, dw, kernels};
 }
 
 class NormFunction : public torch::autograd::Function<NormFunction> {
@@ -175,8 +176,8 @@ class NormFunction : public torch::autograd::Function<NormFunction> {
       auto again = differentiable("_norm_again", 2, saved[0], saved[1], eps, grads[0], some(ds));
       return {again[0], again[1], residual ? again[0] : Tensor(), Tensor()};
     }
-    auto [dx, dw] = rms_norm_bwd(grads[0], some(ds), saved[0], saved[1], eps);
-    g_backward_kernels += kNormBackwardKernels;
+    auto [dx, dw, launches] = rms_norm_bwd(grads[0], some(ds), saved[0], saved[1], eps);
+    g_backward_kernels += launches;
     return {dx, dw, residual ? dx : Tensor(), Tensor()};
   }
 };
@@ -494,7 +495,6 @@ void register_lm(pybind11::module& m) {
   m.def("rms_norm", &rms_norm);
   m.def("gated_scan", &gated_scan);
   m.def("backward_kernels", &backward_kernels);
-  m.attr("NORM_BACKWARD_KERNELS") = kNormBackwardKernels;
   m.def("rms_norm_fwd", &rms_norm_fwd);
   m.def("rms_norm_bwd", &rms_norm_bwd);
   m.def("rms_norm_8bit", &rms_norm_8bit);

@@ -5,7 +5,10 @@
 //   8 bits: scale = max |y| / 448, code = e4m3(y / scale)
 //   dx = ds + rstd * (g - n * mean(g n)),  dw = sum over rows of dy * n,  with g = dy * w, n = s * rstd
 //
-// Sums are fp32. Memory-bound: a few operations for each element that is read and written once.
+// Sums are fp32. Memory-bound: a few operations for each element that is read and written once. A row stays in the registers of the 32 to
+// 512 threads that share it (16 bytes a piece, or an element where rows do not start on 16 bytes), so that it is read once; thread
+// groups walk along the rows with the weight, and backward the weight's gradient, of their columns in registers too. Rows wider than
+// that are read again for every sum.
 #include "rms_norm.h"
 
 #include <cuda_bf16.h>
@@ -48,9 +51,279 @@ __device__ __forceinline__ float block_all(float v, float* shared, Op op) {
   return v;
 }
 
-// A block per row; QUANT: rows leave in 8 bits. The row is read again where it is needed again.
+// ------------------------------------------------------------------------------------------------ rows in registers
+// VEC neighbouring elements as they lie in memory.
+template <typename T, int VEC> struct Piece;
+template <> struct Piece<bf16, 8> {
+  typedef uint4 Raw;
+  static __device__ __forceinline__ Raw load(const bf16* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
+  static __device__ __forceinline__ void unpack(const Raw& r, float* v) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+  }
+  static __device__ __forceinline__ void store(bf16* p, const float* v) {
+    uint4 r;
+    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<uint4*>(p) = r;
+  }
+};
+template <> struct Piece<float, 4> {
+  typedef float4 Raw;
+  static __device__ __forceinline__ Raw load(const float* p) { return __ldg(reinterpret_cast<const float4*>(p)); }
+  static __device__ __forceinline__ void unpack(const Raw& r, float* v) { v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w; }
+  static __device__ __forceinline__ void store(float* p, const float* v) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+};
+template <typename T> struct Piece<T, 1> {
+  typedef T Raw;
+  static __device__ __forceinline__ Raw load(const T* p) { return *p; }
+  static __device__ __forceinline__ void unpack(const Raw& r, float* v) { v[0] = to_f(r); }
+  static __device__ __forceinline__ void store(T* p, const float* v) { *p = from_f<T>(v[0]); }
+};
+template <int VEC, typename W> __device__ __forceinline__ void load_weight(const W* w, float* v) {
+  if constexpr (VEC == 1) {
+    v[0] = to_f(*w);
+  } else if constexpr (sizeof(W) == 2) {
+    Piece<bf16, 8>::unpack(Piece<bf16, 8>::load(w), v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 4) Piece<float, 4>::unpack(Piece<float, 4>::load(w + i), v + i);
+  }
+}
+// e4m3 codes of v * scale
+template <int VEC> __device__ __forceinline__ void store_codes(uint8_t* p, const float* v, float scale) {
+  if constexpr (VEC == 1) {
+    *p = __nv_cvt_float_to_fp8(v[0] * scale, __NV_SATFINITE, __NV_E4M3);
+  } else {
+    uint32_t w[VEC / 4];
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i) {
+      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i] * scale, v[4 * i + 1] * scale), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i + 2] * scale, v[4 * i + 3] * scale), __NV_SATFINITE, __NV_E4M3);
+      w[i] = lo | hi << 16;
+    }
+    if constexpr (VEC == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(p) = w[0];
+  }
+}
+
+// One value from all threads of a row's group (`group` threads, a multiple of 32). `shared`: a float per warp, used by one reduction after
+// another in turns of two.
+template <class Op>
+__device__ __forceinline__ float group_all(float v, int group, float (*shared)[16], int& turn, Op op) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+  if (group == 32) return v;
+  float* s = shared[turn ^= 1];
+  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+  __syncthreads();
+  const int first = threadIdx.x / group * (group / 32);
+  v = s[first];
+  for (int w = 1; w < group / 32; ++w) v = op(v, s[first + w]);
+  return v;
+}
+
+template <typename T, typename W, int VEC, int NV, bool QUANT>
+__global__ void __launch_bounds__(512) norm_kernel(const NormRows p, T* __restrict__ y, uint8_t* __restrict__ codes, long long codes_ld, float* __restrict__ scales,
+                                                    const int group) {
+  typedef Piece<T, VEC> P;
+  __shared__ float shared[2][16];
+  pdl_sync();
+  const int beside = blockDim.x / group, mine = threadIdx.x % group;
+  const float inv_width = 1.0f / p.width;
+  int turn = 0;
+  float w[NV][VEC];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = (mine + k * group) * VEC;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) w[k][j] = 1.0f;
+    if (p.weight != nullptr && c < p.width) load_weight<VEC>(static_cast<const W*>(p.weight) + c, w[k]);
+  }
+  // every thread goes as often as the block's first group: the sums synchronise
+  for (long long base = (long long)blockIdx.x * beside; base < p.rows; base += (long long)gridDim.x * beside) {
+    const long long row = base + threadIdx.x / group;
+    const bool there = row < p.rows;
+    typename P::Raw xr[NV], rr[NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (mine + k * group) * VEC;
+      if (there && c < p.width) {
+        xr[k] = P::load(static_cast<const T*>(p.x) + row * p.x_ld + c);
+        if (p.res != nullptr) rr[k] = P::load(static_cast<const T*>(p.res) + row * p.res_ld + c);
+      }
+    }
+    float v[NV][VEC];
+    float q = 0.f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (mine + k * group) * VEC;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[k][j] = 0.f;
+      if (there && c < p.width) {
+        P::unpack(xr[k], v[k]);
+        if (p.res != nullptr) {
+          float r[VEC];
+          P::unpack(rr[k], r);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) v[k][j] = to_f(from_f<T>(v[k][j] + r[j]));
+          P::store(static_cast<T*>(p.sum) + row * p.width + c, v[k]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) q = fmaf(v[k][j], v[k][j], q);
+    }
+    float rstd = 1.0f;
+    if (p.weight != nullptr) rstd = rsqrtf(group_all(q, group, shared, turn, Add()) * inv_width + p.eps);
+    float most = 0.f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (mine + k * group) * VEC;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        v[k][j] = v[k][j] * rstd * w[k][j];
+        if (QUANT) most = max_nan(most, fabsf(v[k][j]));       // columns that are not there hold zeros, or the row's NaN
+      }
+      if (!QUANT && there && c < p.width) P::store(y + row * p.width + c, v[k]);
+    }
+    if (QUANT) {
+      const float scale = group_all(most, group, shared, turn, Max()) / kE4m3Max;
+      const float inv = scale == 0.f ? 0.f : 1.0f / scale;
+      if (there && mine == 0) scales[row] = scale;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (mine + k * group) * VEC;
+        if (there && c < p.width) store_codes<VEC>(codes + row * codes_ld + c, v[k], inv);
+      }
+    }
+  }
+}
+
+// Gradients of rows and, in part[block], of the weight over the block's rows. A thread's next row is requested before the current one's sums.
+template <typename T, typename W, int VEC, int NV>
+__global__ void __launch_bounds__(512) norm_bwd_kernel(const NormGrad p, const int group) {
+  typedef Piece<T, VEC> P;
+  extern __shared__ float sums[];            // of several groups: [group][width]
+  __shared__ float shared_q[2][16], shared_d[2][16];
+  pdl_sync();
+  const int beside = blockDim.x / group, mine = threadIdx.x % group;
+  const float inv_width = 1.0f / p.width;
+  int turn_q = 0, turn_d = 0;
+  float w[NV][VEC], dw[NV][VEC];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = (mine + k * group) * VEC;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) w[k][j] = dw[k][j] = 0.f;
+    if (c < p.width) load_weight<VEC>(static_cast<const W*>(p.weight) + c, w[k]);
+  }
+  typename P::Raw sr[NV], yr[NV], ar[NV];
+  auto request = [&](long long row) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (mine + k * group) * VEC;
+      if (row < p.rows && c < p.width) {
+        sr[k] = P::load(static_cast<const T*>(p.s) + row * p.s_ld + c);
+        yr[k] = P::load(static_cast<const T*>(p.dy) + row * p.dy_ld + c);
+        if (p.ds != nullptr) ar[k] = P::load(static_cast<const T*>(p.ds) + row * p.ds_ld + c);
+      }
+    }
+  };
+  const long long step = (long long)gridDim.x * beside;
+  long long row = (long long)blockIdx.x * beside + threadIdx.x / group;
+  request(row);
+  for (long long base = (long long)blockIdx.x * beside; base < p.rows; base += step, row += step) {
+    const bool there = row < p.rows;
+    float s[NV][VEC], g[NV][VEC];
+    typename P::Raw add[NV];
+    float q = 0.f, d = 0.f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (mine + k * group) * VEC;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) s[k][j] = g[k][j] = 0.f;
+      if (there && c < p.width) {
+        P::unpack(sr[k], s[k]);
+        P::unpack(yr[k], g[k]);
+        add[k] = ar[k];
+      }
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        q = fmaf(s[k][j], s[k][j], q);
+        d = fmaf(s[k][j] * g[k][j], w[k][j], d);
+      }
+    }
+    request(row + step);
+    q = group_all(q, group, shared_q, turn_q, Add());
+    d = group_all(d, group, shared_d, turn_d, Add());
+    const float rstd = rsqrtf(q * inv_width + p.eps), along = d * rstd * inv_width * rstd;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (mine + k * group) * VEC;
+      float o[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) o[j] = 0.f;
+      if (p.ds != nullptr && there && c < p.width) P::unpack(add[k], o);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float n = s[k][j] * rstd;
+        dw[k][j] = fmaf(g[k][j], n, dw[k][j]);
+        o[j] = fmaf(g[k][j] * w[k][j], rstd, fmaf(-n, along, o[j]));
+      }
+      if (there && c < p.width) P::store(static_cast<T*>(p.dx) + row * p.width + c, o);
+    }
+  }
+  float* part = p.part + (long long)blockIdx.x * p.width;
+  if (beside == 1) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (mine + k * group) * VEC;
+      if (c < p.width)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) part[c + j] = dw[k][j];
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (mine + k * group) * VEC;
+      if (c < p.width)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) sums[threadIdx.x / group * p.width + c + j] = dw[k][j];
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < p.width; c += blockDim.x) {
+      float sum = sums[c];
+      for (int b = 1; b < beside; ++b) sum += sums[b * p.width + c];
+      part[c] = sum;
+    }
+  }
+}
+
+// dw = the sum of the parts: 32 columns a block, its warps a share of the parts each.
+template <typename W>
+__global__ void __launch_bounds__(256) norm_dw_sum_kernel(const float* __restrict__ part, W* __restrict__ dw, int parts, int width) {
+  __shared__ float shared[8][33];
+  pdl_sync();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  float sum = 0.f;
+  if (c < width)
+#pragma unroll 8
+    for (int k = warp; k < parts; k += 8) sum += part[(long long)k * width + c];
+  shared[warp][lane] = sum;
+  __syncthreads();
+  if (warp == 0 && c < width) {
+#pragma unroll
+    for (int k = 1; k < 8; ++k) sum += shared[k][lane];
+    dw[c] = from_f<W>(sum);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ wide rows
+// Wide rows. A block per row; QUANT: rows leave in 8 bits.
 template <typename T, typename W, bool QUANT>
-__global__ void __launch_bounds__(kThreads) norm_kernel(const NormRows p, T* __restrict__ y, uint8_t* __restrict__ codes, long long codes_ld,
+__global__ void __launch_bounds__(kThreads) wide_norm_kernel(const NormRows p, T* __restrict__ y, uint8_t* __restrict__ codes, long long codes_ld,
                                                         float* __restrict__ scales) {
   pdl_sync();
   __shared__ float shared[kThreads / 32];
@@ -90,7 +363,7 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const NormRows p, T* __r
 }
 
 template <typename T, typename W>
-__global__ void __launch_bounds__(kThreads) norm_dx_kernel(const NormGrad p, float* __restrict__ rstds) {
+__global__ void __launch_bounds__(kThreads) wide_norm_dx_kernel(const NormGrad p, float* __restrict__ rstds) {
   pdl_sync();
   __shared__ float shared[kThreads / 32];
   const W* w = static_cast<const W*>(p.weight);
@@ -117,7 +390,7 @@ __global__ void __launch_bounds__(kThreads) norm_dx_kernel(const NormGrad p, flo
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) norm_dw_kernel(const NormGrad p, const float* __restrict__ rstds, float* __restrict__ part, int parts) {
+__global__ void __launch_bounds__(kThreads) wide_norm_dw_kernel(const NormGrad p, const float* __restrict__ rstds, float* __restrict__ part, int parts) {
   pdl_sync();
   const int c = blockIdx.x * kThreads + threadIdx.x;
   if (c >= p.width) return;
@@ -127,21 +400,62 @@ __global__ void __launch_bounds__(kThreads) norm_dw_kernel(const NormGrad p, con
   part[(long long)blockIdx.y * p.width + c] = sum;
 }
 
-template <typename W>
-__global__ void __launch_bounds__(kThreads) norm_dw_sum_kernel(const float* __restrict__ part, W* __restrict__ dw, int parts, int width) {
-  pdl_sync();
-  const int c = blockIdx.x * kThreads + threadIdx.x;
-  if (c >= width) return;
-  float sum = 0.f;
-  for (int k = 0; k < parts; ++k) sum += part[(long long)k * width + c];
-  dw[c] = from_f<W>(sum);
+// ------------------------------------------------------------------------------------------------ host
+// How many pieces a thread holds and how many threads share a row: two pieces each where the rows alone fill the SMs (fewer threads to
+// join for each sum), one where a row's latency counts.
+struct Layout { int pieces, group; };       // pieces 0: the row does not fit
+Layout layout_of(long long rows, int width, int vec, int most_pieces) {
+  const int all = (width + vec - 1) / vec;
+  auto group_for = [&](int pieces) {
+    int g = 32;
+    while (g < 512 && g * pieces < all) g *= 2;
+    return g;
+  };
+  int pieces = vec == 1 ? 4 : rows >= 4LL * sm_count() ? 2 : 1;
+  while (pieces < most_pieces && group_for(pieces) * pieces < all) pieces *= 2;
+  const int group = group_for(pieces);
+  return group * pieces < all ? Layout{0, 0} : Layout{pieces, group};
+}
+int block_of(int group) { return group < 256 ? 256 : group; }
+
+bool aligned(const void* p, long long ld, int bytes) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * bytes % 16 == 0; }
+bool in_pieces(const NormRows& p) {
+  const int size = p.bf16 ? 2 : 4;
+  return aligned(p.x, p.x_ld, size) && aligned(p.res, p.res_ld, size) && aligned(p.sum, p.width, size) && aligned(p.weight, 0, 1) && p.width * size % 16 == 0;
+}
+bool in_pieces(const NormGrad& p) {
+  const int size = p.bf16 ? 2 : 4;
+  return aligned(p.s, p.s_ld, size) && aligned(p.dy, p.dy_ld, size) && aligned(p.ds, p.ds_ld, size) && aligned(p.dx, p.width, size) && aligned(p.weight, 0, 1) &&
+         p.width * size % 16 == 0;
 }
 
+template <typename T, typename W, bool QUANT, int VEC>
+cudaError_t forward_rows(const NormRows& p, const Layout& l, void* y, void* codes, long long codes_ld, float* scales, cudaStream_t st) {
+  const int block = block_of(l.group), beside = block / l.group;
+  const long long blocks = (p.rows + beside - 1) / beside, most = (long long)sm_count() * (2048 / block);
+  auto with = [&](auto kernel) {
+    return launch_pdl(kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(block), 0, st, p, static_cast<T*>(y), static_cast<uint8_t*>(codes), codes_ld, scales,
+                      l.group);
+  };
+  if constexpr (VEC > 1) {
+    if (l.pieces == 1) return with(norm_kernel<T, W, VEC, 1, QUANT>);
+    if (l.pieces == 2) return with(norm_kernel<T, W, VEC, 2, QUANT>);
+    return with(norm_kernel<T, W, VEC, 4, QUANT>);
+  } else {
+    if (l.pieces == 4) return with(norm_kernel<T, W, VEC, 4, QUANT>);
+    return l.pieces == 8 ? with(norm_kernel<T, W, VEC, 8, QUANT>) : with(norm_kernel<T, W, VEC, 16, QUANT>);
+  }
+}
 template <typename T, typename W, bool QUANT>
 cudaError_t forward(const NormRows& p, void* y, void* codes, long long codes_ld, float* scales, cudaStream_t st) {
   if (p.rows <= 0) return cudaSuccess;
+  constexpr int VEC = 16 / sizeof(T);
+  const bool pieces = in_pieces(p) && aligned(y, p.width, sizeof(T));
+  const Layout l = layout_of(p.rows, p.width, pieces ? VEC : 1, pieces ? 4 : 16);
+  if (l.pieces != 0)
+    return pieces ? forward_rows<T, W, QUANT, VEC>(p, l, y, codes, codes_ld, scales, st) : forward_rows<T, W, QUANT, 1>(p, l, y, codes, codes_ld, scales, st);
   const long long most = 8LL * sm_count();
-  return launch_pdl(norm_kernel<T, W, QUANT>, dim3((unsigned)(p.rows < most ? p.rows : most)), dim3(kThreads), 0, st, p, static_cast<T*>(y),
+  return launch_pdl(wide_norm_kernel<T, W, QUANT>, dim3((unsigned)(p.rows < most ? p.rows : most)), dim3(kThreads), 0, st, p, static_cast<T*>(y),
                     static_cast<uint8_t*>(codes), codes_ld, scales);
 }
 template <bool QUANT>
@@ -150,21 +464,54 @@ cudaError_t forward_of(const NormRows& p, void* y, void* codes, long long codes_
   return p.weight_bf16 ? forward<bf16, bf16, QUANT>(p, y, codes, codes_ld, scales, st) : forward<bf16, float, QUANT>(p, y, codes, codes_ld, scales, st);
 }
 
-constexpr int kParts = 64;
+constexpr int kWideParts = 64;
+constexpr int kBlocksBack = 2;               // on an SM
 
-template <typename T, typename W>
-cudaError_t backward(const NormGrad& p, cudaStream_t st) {
-  const int parts = rms_norm_bwd_parts(p.rows, p.width) - (int)((p.rows + p.width - 1) / p.width);
-  float* rstds = p.part + (long long)parts * p.width;
-  const unsigned cols = (p.width + kThreads - 1) / kThreads;
-  cudaError_t e = cudaSuccess;
-  if (p.rows > 0) {
-    const long long most = 8LL * sm_count();
-    e = launch_pdl(norm_dx_kernel<T, W>, dim3((unsigned)(p.rows < most ? p.rows : most)), dim3(kThreads), 0, st, p, rstds);
-    if (e == cudaSuccess) e = launch_pdl(norm_dw_kernel<T>, dim3(cols, parts), dim3(kThreads), 0, st, p, rstds, p.part, parts);
+Layout layout_back(const NormGrad& p) {
+  const bool pieces = in_pieces(p);
+  return layout_of(pieces ? p.rows : 0, p.width, pieces ? (p.bf16 ? 8 : 4) : 1, pieces ? 4 : 16);
+}
+int blocks_back(const NormGrad& p, const Layout& l) {
+  const int beside = block_of(l.group) / l.group;
+  const long long blocks = (p.rows + beside - 1) / beside, most = (long long)sm_count() * kBlocksBack;
+  return (int)(blocks < most ? blocks : most);
+}
+
+template <typename T, typename W, int VEC>
+cudaError_t backward_rows(const NormGrad& p, const Layout& l, cudaStream_t st) {
+  const int block = block_of(l.group), beside = block / l.group;
+  const size_t smem = beside > 1 ? (size_t)beside * p.width * sizeof(float) : 0;
+  auto with = [&](auto kernel) { return launch_pdl(kernel, dim3(blocks_back(p, l)), dim3(block), smem, st, p, l.group); };
+  if constexpr (VEC > 1) {
+    if (l.pieces == 1) return with(norm_bwd_kernel<T, W, VEC, 1>);
+    if (l.pieces == 2) return with(norm_bwd_kernel<T, W, VEC, 2>);
+    return with(norm_bwd_kernel<T, W, VEC, 4>);
+  } else {
+    if (l.pieces == 4) return with(norm_bwd_kernel<T, W, VEC, 4>);
+    return l.pieces == 8 ? with(norm_bwd_kernel<T, W, VEC, 8>) : with(norm_bwd_kernel<T, W, VEC, 16>);
   }
-  if (e == cudaSuccess) e = launch_pdl(norm_dw_sum_kernel<W>, dim3(cols), dim3(kThreads), 0, st, p.part, static_cast<W*>(p.dw), p.rows > 0 ? parts : 0, p.width);
-  return e;
+}
+template <typename T, typename W>
+cudaError_t backward(const NormGrad& p, int* launched, cudaStream_t st) {
+  const Layout l = layout_back(p);
+  int parts = 0;
+  cudaError_t e = cudaSuccess;
+  *launched = 1;
+  if (p.rows > 0 && l.pieces != 0) {
+    parts = blocks_back(p, l);
+    *launched = 2;
+    e = in_pieces(p) ? backward_rows<T, W, 16 / sizeof(T)>(p, l, st) : backward_rows<T, W, 1>(p, l, st);
+  } else if (p.rows > 0) {
+    parts = kWideParts;
+    *launched = 3;
+    float* rstds = p.part + (long long)parts * p.width;
+    const long long most = 8LL * sm_count();
+    e = launch_pdl(wide_norm_dx_kernel<T, W>, dim3((unsigned)(p.rows < most ? p.rows : most)), dim3(kThreads), 0, st, p, rstds);
+    if (e == cudaSuccess)
+      e = launch_pdl(wide_norm_dw_kernel<T>, dim3((p.width + kThreads - 1) / kThreads, parts), dim3(kThreads), 0, st, p, rstds, p.part, parts);
+  }
+  if (e != cudaSuccess) return e;
+  return launch_pdl(norm_dw_sum_kernel<W>, dim3((p.width + 31) / 32), dim3(256), 0, st, p.part, static_cast<W*>(p.dw), parts, p.width);
 }
 
 }  // namespace
@@ -173,10 +520,13 @@ cudaError_t rms_norm_fwd(const NormRows& p, void* y, cudaStream_t st) { return f
 cudaError_t rms_norm_8bit(const NormRows& p, void* codes, long long codes_ld, float* scales, cudaStream_t st) {
   return forward_of<true>(p, nullptr, codes, codes_ld, scales, st);
 }
-int rms_norm_bwd_parts(long long rows, int width) { return kParts + (int)((rows + width - 1) / width); }      // the rows' rstd behind the sums
-cudaError_t rms_norm_bwd(const NormGrad& p, cudaStream_t st) {
-  if (!p.bf16) return p.weight_bf16 ? cudaErrorInvalidValue : backward<float, float>(p, st);
-  return p.weight_bf16 ? backward<bf16, bf16>(p, st) : backward<bf16, float>(p, st);
+long long rms_norm_bwd_floats(const NormGrad& p) {
+  const Layout l = layout_back(p);
+  return l.pieces != 0 ? (long long)blocks_back(p, l) * p.width : (long long)kWideParts * p.width + p.rows;       // the rows' rstd behind the sums
+}
+cudaError_t rms_norm_bwd(const NormGrad& p, int* launched, cudaStream_t st) {
+  if (!p.bf16) return p.weight_bf16 ? cudaErrorInvalidValue : backward<float, float>(p, launched, st);
+  return p.weight_bf16 ? backward<bf16, bf16>(p, launched, st) : backward<bf16, float>(p, launched, st);
 }
 
 }  // namespace adb200

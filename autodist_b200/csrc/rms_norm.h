@@ -25,12 +25,13 @@ struct NormGrad {
   const void* s; long long s_ld;            // what was normed
   const void* weight;
   void* dx;                                 // [rows, width]
-  float* part;                              // rms_norm_bwd_parts(rows, width) x width
+  float* part;                              // rms_norm_bwd_floats(p)
   void* dw;                                 // [width] of the weight's type
   long long rows; int width; float eps;
   bool bf16, weight_bf16;
 };
-int rms_norm_bwd_parts(long long rows, int width);
-cudaError_t rms_norm_bwd(const NormGrad& p, cudaStream_t st);
+// Floats of scratch (all but `part` and `dw` have to be set); launched: how many kernels it took.
+long long rms_norm_bwd_floats(const NormGrad& p);
+cudaError_t rms_norm_bwd(const NormGrad& p, int* launched, cudaStream_t st);
 
 }  // namespace adb200
