@@ -14,6 +14,9 @@
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
+#include <mutex>
+#include <set>
+
 #include "pdl.cuh"
 #include "sm_count.h"
 
@@ -92,16 +95,15 @@ template <int VEC, typename W> __device__ __forceinline__ void load_weight(const
     for (int i = 0; i < VEC; i += 4) Piece<float, 4>::unpack(Piece<float, 4>::load(w + i), v + i);
   }
 }
-// e4m3 codes of v * scale
-template <int VEC> __device__ __forceinline__ void store_codes(uint8_t* p, const float* v, float scale) {
+template <int VEC> __device__ __forceinline__ void store_codes(uint8_t* p, const float* v) {
   if constexpr (VEC == 1) {
-    *p = __nv_cvt_float_to_fp8(v[0] * scale, __NV_SATFINITE, __NV_E4M3);
+    *p = __nv_cvt_float_to_fp8(v[0], __NV_SATFINITE, __NV_E4M3);
   } else {
     uint32_t w[VEC / 4];
 #pragma unroll
     for (int i = 0; i < VEC / 4; ++i) {
-      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i] * scale, v[4 * i + 1] * scale), __NV_SATFINITE, __NV_E4M3);
-      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i + 2] * scale, v[4 * i + 3] * scale), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i], v[4 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i + 2], v[4 * i + 3]), __NV_SATFINITE, __NV_E4M3);
       w[i] = lo | hi << 16;
     }
     if constexpr (VEC == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
@@ -109,19 +111,76 @@ template <int VEC> __device__ __forceinline__ void store_codes(uint8_t* p, const
   }
 }
 
-// One value from all threads of a row's group (`group` threads, a multiple of 32). `shared`: a float per warp, used by one reduction after
-// another in turns of two.
-template <class Op>
-__device__ __forceinline__ float group_all(float v, int group, float (*shared)[16], int& turn, Op op) {
+// A thread's pieces of its next AT - 1 rows come ahead of it into shared memory, where 16 bytes of a thread lie beside the next thread's:
+// it reads what it asked for itself, so nothing synchronises. Elements by themselves are read when their row's turn comes.
+template <typename T, int VEC, int NV, int NT>
+struct Rows {
+  typedef Piece<T, VEC> P;
+  static constexpr bool AHEAD = VEC > 1;
+  static constexpr int AT = NV > 2 ? 2 : 4;
+  static constexpr int THREAD = AHEAD ? AT * NT * NV * 16 : 0;             // bytes of shared memory
+  uint8_t* ring;
+  typename P::Raw now[AHEAD ? 1 : NT][AHEAD ? 1 : NV];                         // elements by themselves: of the row that comes next
+  __device__ __forceinline__ explicit Rows(uint8_t* shared) : ring(shared + threadIdx.x * 16) {}
+  __device__ __forceinline__ uint8_t* slot(int stage, int tensor, int k) const { return ring + ((stage * NT + tensor) * NV + k) * (int)blockDim.x * 16; }
+  // tensors t of row `row`, columns of piece k from (mine + k * group) * VEC on
+  __device__ __forceinline__ void request(int stage, const T* const* from, bool there, int mine, int group, int width) {
+    if constexpr (AHEAD) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+          const int c = (mine + k * group) * VEC;
+          if (there && from[t] != nullptr && c < width)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(slot(stage, t, k))), "l"(from[t] + c) : "memory");
+        }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+  }
+  __device__ __forceinline__ void arrived() const {
+    if constexpr (AHEAD) asm volatile("cp.async.wait_group %0;" ::"n"(AT - 1) : "memory");
+  }
+  // elements by themselves: the next row, once the current one has been read
+  __device__ __forceinline__ void fetch(const T* const* from, bool there, int mine, int group, int width) {
+    if constexpr (!AHEAD) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+          const int c = (mine + k * group) * VEC;
+          if (there && from[t] != nullptr && c < width) now[t][k] = P::load(from[t] + c);
+        }
+    }
+  }
+  __device__ __forceinline__ void all_arrived() const {
+    if constexpr (AHEAD) asm volatile("cp.async.wait_group 0;" ::: "memory");
+  }
+  __device__ __forceinline__ void read(int stage, int tensor, int k, float* v) const {
+    if constexpr (AHEAD) P::unpack(*reinterpret_cast<const typename P::Raw*>(slot(stage, tensor, k)), v);
+    else P::unpack(now[tensor][k], v);
+  }
+};
+
+// Two values from all threads of a row's group (`group` threads, a multiple of 32), in one exchange. `shared`: a pair per warp, used by one
+// exchange after another in turns of two.
+template <class Op, class Op2>
+__device__ __forceinline__ float2 group_all(float2 v, int group, float2 (*shared)[16], int& turn, Op op, Op2 op2) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    v.x = op(v.x, __shfl_xor_sync(0xffffffffu, v.x, o));
+    v.y = op2(v.y, __shfl_xor_sync(0xffffffffu, v.y, o));
+  }
   if (group == 32) return v;
-  float* s = shared[turn ^= 1];
+  float2* s = shared[turn ^= 1];
   if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
   __syncthreads();
   const int first = threadIdx.x / group * (group / 32);
   v = s[first];
-  for (int w = 1; w < group / 32; ++w) v = op(v, s[first + w]);
+  for (int w = 1; w < group / 32; ++w) {
+    const float2 u = s[first + w];
+    v.x = op(v.x, u.x);
+    v.y = op2(v.y, u.y);
+  }
   return v;
 }
 
@@ -129,7 +188,8 @@ template <typename T, typename W, int VEC, int NV, bool QUANT>
 __global__ void __launch_bounds__(512) norm_kernel(const NormRows p, T* __restrict__ y, uint8_t* __restrict__ codes, long long codes_ld, float* __restrict__ scales,
                                                     const int group) {
   typedef Piece<T, VEC> P;
-  __shared__ float shared[2][16];
+  extern __shared__ __align__(16) uint8_t ahead[];
+  __shared__ float2 shared[2][16];
   pdl_sync();
   const int beside = blockDim.x / group, mine = threadIdx.x % group;
   const float inv_width = 1.0f / p.width;
@@ -142,75 +202,81 @@ __global__ void __launch_bounds__(512) norm_kernel(const NormRows p, T* __restri
     for (int j = 0; j < VEC; ++j) w[k][j] = 1.0f;
     if (p.weight != nullptr && c < p.width) load_weight<VEC>(static_cast<const W*>(p.weight) + c, w[k]);
   }
-  // every thread goes as often as the block's first group: the sums synchronise
-  for (long long base = (long long)blockIdx.x * beside; base < p.rows; base += (long long)gridDim.x * beside) {
-    const long long row = base + threadIdx.x / group;
-    const bool there = row < p.rows;
-    typename P::Raw xr[NV], rr[NV];
+  Rows<T, VEC, NV, 2> rows(ahead);
+  constexpr int AT = rows.AT;
+  const long long step = (long long)gridDim.x * beside;
+  long long row = (long long)blockIdx.x * beside + threadIdx.x / group;
+  struct From { const T* at[2]; };
+  auto from = [&](long long r) {
+    return From{{static_cast<const T*>(p.x) + r * p.x_ld, p.res != nullptr ? static_cast<const T*>(p.res) + r * p.res_ld : nullptr}};
+  };
+  auto request = [&](int stage, long long r) { rows.request(stage, from(r).at, r < p.rows, mine, group, p.width); };
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int c = (mine + k * group) * VEC;
-      if (there && c < p.width) {
-        xr[k] = P::load(static_cast<const T*>(p.x) + row * p.x_ld + c);
-        if (p.res != nullptr) rr[k] = P::load(static_cast<const T*>(p.res) + row * p.res_ld + c);
-      }
-    }
+  for (int k = 0; k < AT - 1; ++k) request(k, row + k * step);
+  rows.fetch(from(row).at, row < p.rows, mine, group, p.width);
+  int stage = 0;
+  // every thread goes as often as the block's first group: the sums synchronise
+  for (long long base = (long long)blockIdx.x * beside; base < p.rows; base += step, row += step, stage = (stage + 1) % AT) {
+    const bool there = row < p.rows;
+    request((stage + AT - 1) % AT, row + (AT - 1) * step);
+    rows.arrived();
     float v[NV][VEC];
-    float q = 0.f;
+    float q = 0.f, most = 0.f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int c = (mine + k * group) * VEC;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) v[k][j] = 0.f;
       if (there && c < p.width) {
-        P::unpack(xr[k], v[k]);
+        rows.read(stage, 0, k, v[k]);
         if (p.res != nullptr) {
           float r[VEC];
-          P::unpack(rr[k], r);
+          rows.read(stage, 1, k, r);
 #pragma unroll
           for (int j = 0; j < VEC; ++j) v[k][j] = to_f(from_f<T>(v[k][j] + r[j]));
           P::store(static_cast<T*>(p.sum) + row * p.width + c, v[k]);
         }
       }
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) q = fmaf(v[k][j], v[k][j], q);
+      for (int j = 0; j < VEC; ++j) {
+        q = fmaf(v[k][j], v[k][j], q);
+        if (QUANT) most = max_nan(most, fabsf(v[k][j] * w[k][j]));
+      }
     }
+    rows.fetch(from(row + step).at, row + step < p.rows, mine, group, p.width);
     float rstd = 1.0f;
-    if (p.weight != nullptr) rstd = rsqrtf(group_all(q, group, shared, turn, Add()) * inv_width + p.eps);
-    float most = 0.f;
+    if (QUANT || p.weight != nullptr) {
+      const float2 r = group_all(make_float2(q, most), group, shared, turn, Add(), Max());
+      if (p.weight != nullptr) rstd = rsqrtf(r.x * inv_width + p.eps);
+      most = r.y;
+    }
+    // the largest size of the products is found beside the sum of squares: rstd, which they share, is one more factor of it
+    const float scale = most * rstd / kE4m3Max, inv = scale == 0.f ? 0.f : rstd / scale;
+    if (QUANT && there && mine == 0) scales[row] = scale;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int c = (mine + k * group) * VEC;
+      const float factor = QUANT ? inv : rstd;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        v[k][j] = v[k][j] * rstd * w[k][j];
-        if (QUANT) most = max_nan(most, fabsf(v[k][j]));       // columns that are not there hold zeros, or the row's NaN
-      }
-      if (!QUANT && there && c < p.width) P::store(y + row * p.width + c, v[k]);
-    }
-    if (QUANT) {
-      const float scale = group_all(most, group, shared, turn, Max()) / kE4m3Max;
-      const float inv = scale == 0.f ? 0.f : 1.0f / scale;
-      if (there && mine == 0) scales[row] = scale;
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int c = (mine + k * group) * VEC;
-        if (there && c < p.width) store_codes<VEC>(codes + row * codes_ld + c, v[k], inv);
+      for (int j = 0; j < VEC; ++j) v[k][j] = v[k][j] * factor * w[k][j];
+      if (there && c < p.width) {
+        if (QUANT) store_codes<VEC>(codes + row * codes_ld + c, v[k]);
+        else P::store(y + row * p.width + c, v[k]);
       }
     }
   }
 }
 
-// Gradients of rows and, in part[block], of the weight over the block's rows. A thread's next row is requested before the current one's sums.
+// Gradients of rows and, in part[block], of the weight over the block's rows.
 template <typename T, typename W, int VEC, int NV>
-__global__ void __launch_bounds__(512) norm_bwd_kernel(const NormGrad p, const int group) {
+__global__ void __launch_bounds__(512, VEC * NV <= 8 ? 2 : 1) norm_bwd_kernel(const NormGrad p, const int group) {
   typedef Piece<T, VEC> P;
-  extern __shared__ float sums[];            // of several groups: [group][width]
-  __shared__ float shared_q[2][16], shared_d[2][16];
+  extern __shared__ __align__(16) uint8_t ahead[];
+  __shared__ float2 shared[2][16];
   pdl_sync();
   const int beside = blockDim.x / group, mine = threadIdx.x % group;
   const float inv_width = 1.0f / p.width;
-  int turn_q = 0, turn_d = 0;
+  int turn = 0;
   float w[NV][VEC], dw[NV][VEC];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
@@ -219,25 +285,24 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const NormGrad p, const i
     for (int j = 0; j < VEC; ++j) w[k][j] = dw[k][j] = 0.f;
     if (c < p.width) load_weight<VEC>(static_cast<const W*>(p.weight) + c, w[k]);
   }
-  typename P::Raw sr[NV], yr[NV], ar[NV];
-  auto request = [&](long long row) {
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int c = (mine + k * group) * VEC;
-      if (row < p.rows && c < p.width) {
-        sr[k] = P::load(static_cast<const T*>(p.s) + row * p.s_ld + c);
-        yr[k] = P::load(static_cast<const T*>(p.dy) + row * p.dy_ld + c);
-        if (p.ds != nullptr) ar[k] = P::load(static_cast<const T*>(p.ds) + row * p.ds_ld + c);
-      }
-    }
-  };
+  Rows<T, VEC, NV, 3> rows(ahead);
+  constexpr int AT = rows.AT;
   const long long step = (long long)gridDim.x * beside;
   long long row = (long long)blockIdx.x * beside + threadIdx.x / group;
-  request(row);
-  for (long long base = (long long)blockIdx.x * beside; base < p.rows; base += step, row += step) {
+  struct From { const T* at[3]; };
+  auto from = [&](long long r) {
+    return From{{static_cast<const T*>(p.s) + r * p.s_ld, static_cast<const T*>(p.dy) + r * p.dy_ld, p.ds != nullptr ? static_cast<const T*>(p.ds) + r * p.ds_ld : nullptr}};
+  };
+  auto request = [&](int stage, long long r) { rows.request(stage, from(r).at, r < p.rows, mine, group, p.width); };
+#pragma unroll
+  for (int k = 0; k < AT - 1; ++k) request(k, row + k * step);
+  rows.fetch(from(row).at, row < p.rows, mine, group, p.width);
+  int stage = 0;
+  for (long long base = (long long)blockIdx.x * beside; base < p.rows; base += step, row += step, stage = (stage + 1) % AT) {
     const bool there = row < p.rows;
+    request((stage + AT - 1) % AT, row + (AT - 1) * step);
+    rows.arrived();
     float s[NV][VEC], g[NV][VEC];
-    typename P::Raw add[NV];
     float q = 0.f, d = 0.f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -245,9 +310,8 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const NormGrad p, const i
 #pragma unroll
       for (int j = 0; j < VEC; ++j) s[k][j] = g[k][j] = 0.f;
       if (there && c < p.width) {
-        P::unpack(sr[k], s[k]);
-        P::unpack(yr[k], g[k]);
-        add[k] = ar[k];
+        rows.read(stage, 0, k, s[k]);
+        rows.read(stage, 1, k, g[k]);
       }
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
@@ -255,17 +319,24 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const NormGrad p, const i
         d = fmaf(s[k][j] * g[k][j], w[k][j], d);
       }
     }
-    request(row + step);
-    q = group_all(q, group, shared_q, turn_q, Add());
-    d = group_all(d, group, shared_d, turn_d, Add());
-    const float rstd = rsqrtf(q * inv_width + p.eps), along = d * rstd * inv_width * rstd;
+    typename P::Raw add[rows.AHEAD ? 1 : NV];
+    if constexpr (!rows.AHEAD) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) add[k] = rows.now[2][k];
+      rows.fetch(from(row + step).at, row + step < p.rows, mine, group, p.width);
+    }
+    const float2 r = group_all(make_float2(q, d), group, shared, turn, Add(), Add());
+    const float rstd = rsqrtf(r.x * inv_width + p.eps), along = r.y * rstd * inv_width * rstd;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int c = (mine + k * group) * VEC;
       float o[VEC];
 #pragma unroll
       for (int j = 0; j < VEC; ++j) o[j] = 0.f;
-      if (p.ds != nullptr && there && c < p.width) P::unpack(add[k], o);
+      if (p.ds != nullptr && there && c < p.width) {
+        if constexpr (rows.AHEAD) rows.read(stage, 2, k, o);
+        else P::unpack(add[k], o);
+      }
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         const float n = s[k][j] * rstd;
@@ -276,6 +347,7 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const NormGrad p, const i
     }
   }
   float* part = p.part + (long long)blockIdx.x * p.width;
+  rows.all_arrived();
   if (beside == 1) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -285,6 +357,8 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const NormGrad p, const i
         for (int j = 0; j < VEC; ++j) part[c + j] = dw[k][j];
     }
   } else {
+    float* sums = reinterpret_cast<float*>(ahead);         // [group][width], where the rows were
+    __syncthreads();
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int c = (mine + k * group) * VEC;
@@ -302,22 +376,22 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const NormGrad p, const i
 }
 
 // dw = the sum of the parts: 32 columns a block, its warps a share of the parts each.
+constexpr int kSumWarps = 32;
 template <typename W>
-__global__ void __launch_bounds__(256) norm_dw_sum_kernel(const float* __restrict__ part, W* __restrict__ dw, int parts, int width) {
-  __shared__ float shared[8][33];
+__global__ void __launch_bounds__(32 * kSumWarps) norm_dw_sum_kernel(const float* __restrict__ part, W* __restrict__ dw, int parts, int width) {
+  __shared__ float shared[kSumWarps][33];
   pdl_sync();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   float sum = 0.f;
   if (c < width)
 #pragma unroll 8
-    for (int k = warp; k < parts; k += 8) sum += part[(long long)k * width + c];
+    for (int k = warp; k < parts; k += kSumWarps) sum += part[(long long)k * width + c];
   shared[warp][lane] = sum;
   __syncthreads();
-  if (warp == 0 && c < width) {
+  sum = shared[lane][warp];                  // column `warp` of the block, part `lane`
 #pragma unroll
-    for (int k = 1; k < 8; ++k) sum += shared[k][lane];
-    dw[c] = from_f<W>(sum);
-  }
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0 && blockIdx.x * 32 + warp < width) dw[blockIdx.x * 32 + warp] = from_f<W>(sum);
 }
 
 // ------------------------------------------------------------------------------------------------ wide rows
@@ -429,21 +503,36 @@ bool in_pieces(const NormGrad& p) {
          p.width * size % 16 == 0;
 }
 
+// More shared memory than a kernel has by itself has to be asked for, once.
+cudaError_t allow(const void* kernel, size_t smem) {
+  if (smem <= 40 * 1024) return cudaSuccess;
+  static std::mutex mutex;
+  static std::set<const void*> asked;
+  const std::lock_guard<std::mutex> lock(mutex);
+  if (asked.count(kernel)) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+  if (e == cudaSuccess) asked.insert(kernel);
+  return e;
+}
+
 template <typename T, typename W, bool QUANT, int VEC>
 cudaError_t forward_rows(const NormRows& p, const Layout& l, void* y, void* codes, long long codes_ld, float* scales, cudaStream_t st) {
   const int block = block_of(l.group), beside = block / l.group;
-  const long long blocks = (p.rows + beside - 1) / beside, most = (long long)sm_count() * (2048 / block);
-  auto with = [&](auto kernel) {
-    return launch_pdl(kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(block), 0, st, p, static_cast<T*>(y), static_cast<uint8_t*>(codes), codes_ld, scales,
+  const long long blocks = (p.rows + beside - 1) / beside, most = (long long)sm_count() * (l.pieces * VEC <= 8 ? 2048 : 768) / block;
+  auto with = [&](auto kernel, int thread) {
+    const size_t smem = (size_t)thread * block;
+    const cudaError_t e = allow(reinterpret_cast<const void*>(kernel), smem);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(block), smem, st, p, static_cast<T*>(y), static_cast<uint8_t*>(codes), codes_ld, scales,
                       l.group);
   };
   if constexpr (VEC > 1) {
-    if (l.pieces == 1) return with(norm_kernel<T, W, VEC, 1, QUANT>);
-    if (l.pieces == 2) return with(norm_kernel<T, W, VEC, 2, QUANT>);
-    return with(norm_kernel<T, W, VEC, 4, QUANT>);
+    if (l.pieces == 1) return with(norm_kernel<T, W, VEC, 1, QUANT>, Rows<T, VEC, 1, 2>::THREAD);
+    if (l.pieces == 2) return with(norm_kernel<T, W, VEC, 2, QUANT>, Rows<T, VEC, 2, 2>::THREAD);
+    return with(norm_kernel<T, W, VEC, 4, QUANT>, Rows<T, VEC, 4, 2>::THREAD);
   } else {
-    if (l.pieces == 4) return with(norm_kernel<T, W, VEC, 4, QUANT>);
-    return l.pieces == 8 ? with(norm_kernel<T, W, VEC, 8, QUANT>) : with(norm_kernel<T, W, VEC, 16, QUANT>);
+    if (l.pieces == 4) return with(norm_kernel<T, W, VEC, 4, QUANT>, Rows<T, VEC, 4, 2>::THREAD);
+    return l.pieces == 8 ? with(norm_kernel<T, W, VEC, 8, QUANT>, Rows<T, VEC, 8, 2>::THREAD) : with(norm_kernel<T, W, VEC, 16, QUANT>, Rows<T, VEC, 16, 2>::THREAD);
   }
 }
 template <typename T, typename W, bool QUANT>
@@ -465,7 +554,7 @@ cudaError_t forward_of(const NormRows& p, void* y, void* codes, long long codes_
 }
 
 constexpr int kWideParts = 64;
-constexpr int kBlocksBack = 2;               // on an SM
+constexpr int kThreadsBack = 512;            // on an SM, twice as many where a thread has 8 columns at most
 
 Layout layout_back(const NormGrad& p) {
   const bool pieces = in_pieces(p);
@@ -473,22 +562,26 @@ Layout layout_back(const NormGrad& p) {
 }
 int blocks_back(const NormGrad& p, const Layout& l) {
   const int beside = block_of(l.group) / l.group;
-  const long long blocks = (p.rows + beside - 1) / beside, most = (long long)sm_count() * kBlocksBack;
+  const long long blocks = (p.rows + beside - 1) / beside, most = (long long)sm_count() * (kThreadsBack / block_of(l.group)) * (l.pieces * (in_pieces(p) ? (p.bf16 ? 8 : 4) : 1) <= 8 ? 2 : 1);
   return (int)(blocks < most ? blocks : most);
 }
 
 template <typename T, typename W, int VEC>
 cudaError_t backward_rows(const NormGrad& p, const Layout& l, cudaStream_t st) {
   const int block = block_of(l.group), beside = block / l.group;
-  const size_t smem = beside > 1 ? (size_t)beside * p.width * sizeof(float) : 0;
-  auto with = [&](auto kernel) { return launch_pdl(kernel, dim3(blocks_back(p, l)), dim3(block), smem, st, p, l.group); };
+  auto with = [&](auto kernel, int thread) {
+    const size_t joined = beside > 1 ? (size_t)beside * p.width * sizeof(float) : 0, ahead = (size_t)thread * block, smem = joined > ahead ? joined : ahead;
+    const cudaError_t e = allow(reinterpret_cast<const void*>(kernel), smem);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(kernel, dim3(blocks_back(p, l)), dim3(block), smem, st, p, l.group);
+  };
   if constexpr (VEC > 1) {
-    if (l.pieces == 1) return with(norm_bwd_kernel<T, W, VEC, 1>);
-    if (l.pieces == 2) return with(norm_bwd_kernel<T, W, VEC, 2>);
-    return with(norm_bwd_kernel<T, W, VEC, 4>);
+    if (l.pieces == 1) return with(norm_bwd_kernel<T, W, VEC, 1>, Rows<T, VEC, 1, 3>::THREAD);
+    if (l.pieces == 2) return with(norm_bwd_kernel<T, W, VEC, 2>, Rows<T, VEC, 2, 3>::THREAD);
+    return with(norm_bwd_kernel<T, W, VEC, 4>, Rows<T, VEC, 4, 3>::THREAD);
   } else {
-    if (l.pieces == 4) return with(norm_bwd_kernel<T, W, VEC, 4>);
-    return l.pieces == 8 ? with(norm_bwd_kernel<T, W, VEC, 8>) : with(norm_bwd_kernel<T, W, VEC, 16>);
+    if (l.pieces == 4) return with(norm_bwd_kernel<T, W, VEC, 4>, Rows<T, VEC, 4, 3>::THREAD);
+    return l.pieces == 8 ? with(norm_bwd_kernel<T, W, VEC, 8>, Rows<T, VEC, 8, 3>::THREAD) : with(norm_bwd_kernel<T, W, VEC, 16>, Rows<T, VEC, 16, 3>::THREAD);
   }
 }
 template <typename T, typename W>
@@ -511,7 +604,7 @@ cudaError_t backward(const NormGrad& p, int* launched, cudaStream_t st) {
       e = launch_pdl(wide_norm_dw_kernel<T>, dim3((p.width + kThreads - 1) / kThreads, parts), dim3(kThreads), 0, st, p, rstds, p.part, parts);
   }
   if (e != cudaSuccess) return e;
-  return launch_pdl(norm_dw_sum_kernel<W>, dim3((p.width + 31) / 32), dim3(256), 0, st, p.part, static_cast<W*>(p.dw), parts, p.width);
+  return launch_pdl(norm_dw_sum_kernel<W>, dim3((p.width + 31) / 32), dim3(32 * kSumWarps), 0, st, p.part, static_cast<W*>(p.dw), parts, p.width);
 }
 
 }  // namespace
