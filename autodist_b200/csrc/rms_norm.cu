@@ -6,7 +6,7 @@
 //   dx = ds + rstd * (g - n * mean(g n)),  dw = sum over rows of dy * n,  with g = dy * w, n = s * rstd
 //
 // Sums are fp32. Memory-bound: a few operations for each element that is read and written once. A row stays in the registers of the 32 to
-// 512 threads that share it (16 bytes a piece, or an element where rows do not start on 16 bytes), so that it is read once; thread
+// 512 threads that share it (16 bytes a piece), so that it is read once; thread
 // groups walk along the rows with the weight, and backward the weight's gradient, of their columns in registers too. Rows wider than
 // that are read again for every sum.
 #include "rms_norm.h"
@@ -79,15 +79,12 @@ template <> struct Piece<float, 4> {
   static __device__ __forceinline__ void unpack(const Raw& r, float* v) { v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w; }
   static __device__ __forceinline__ void store(float* p, const float* v) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
 };
-template <typename T> struct Piece<T, 1> {
-  typedef T Raw;
-  static __device__ __forceinline__ Raw load(const T* p) { return *p; }
-  static __device__ __forceinline__ void unpack(const Raw& r, float* v) { v[0] = to_f(r); }
-  static __device__ __forceinline__ void store(T* p, const float* v) { *p = from_f<T>(v[0]); }
-};
-template <int VEC, typename W> __device__ __forceinline__ void load_weight(const W* w, float* v) {
-  if constexpr (VEC == 1) {
-    v[0] = to_f(*w);
+// columns c ... of the weight, zeros where there are none
+template <int VEC, bool SHIFT, typename W> __device__ __forceinline__ void load_weight(const W* w, int c, int width, float* v) {
+  w += c;
+  if constexpr (SHIFT) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = c + j >= 0 && c + j < width ? to_f(w[j]) : 0.f;
   } else if constexpr (sizeof(W) == 2) {
     Piece<bf16, 8>::unpack(Piece<bf16, 8>::load(w), v);
   } else {
@@ -95,9 +92,12 @@ template <int VEC, typename W> __device__ __forceinline__ void load_weight(const
     for (int i = 0; i < VEC; i += 4) Piece<float, 4>::unpack(Piece<float, 4>::load(w + i), v + i);
   }
 }
-template <int VEC> __device__ __forceinline__ void store_codes(uint8_t* p, const float* v) {
-  if constexpr (VEC == 1) {
-    *p = __nv_cvt_float_to_fp8(v[0], __NV_SATFINITE, __NV_E4M3);
+template <int VEC, bool SHIFT> __device__ __forceinline__ void store_codes(uint8_t* p, int c, int width, const float* v) {
+  p += c;
+  if constexpr (SHIFT) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j)
+      if (c + j >= 0 && c + j < width) p[j] = __nv_cvt_float_to_fp8(v[j], __NV_SATFINITE, __NV_E4M3);
   } else {
     uint32_t w[VEC / 4];
 #pragma unroll
@@ -111,53 +111,73 @@ template <int VEC> __device__ __forceinline__ void store_codes(uint8_t* p, const
   }
 }
 
+// How rows lie. In all three a thread has the same columns of a row, so that a row's sums have the same bits:
+//   kAligned  whole pieces of 16 bytes
+//   kShifted  rows of any width one after the other: their pieces start up to VEC - 1 elements in front of the row. A group's rows are a
+//             multiple of VEC apart, so that all of them, and with them the columns of its threads, are shifted alike; what a piece
+//             holds of the rows beside is left out
+//   kSingle   anything else, element by element
+enum Kind { kAligned, kShifted, kSingle };
+
 // A thread's pieces of its next AT - 1 rows come ahead of it into shared memory, where 16 bytes of a thread lie beside the next thread's:
-// it reads what it asked for itself, so nothing synchronises. Elements by themselves are read when their row's turn comes.
-template <typename T, int VEC, int NV, int NT>
+// it reads what it asked for itself, so nothing synchronises. Single elements are read when their row's turn comes.
+template <typename T, int VEC, int NV, int NT, int KIND>
 struct Rows {
   typedef Piece<T, VEC> P;
-  static constexpr bool AHEAD = VEC > 1;
-  static constexpr int AT = NV > 2 ? 2 : 4;
-  static constexpr int THREAD = AHEAD ? AT * NT * NV * 16 : 0;             // bytes of shared memory
+  static constexpr int AT = NV > 2 ? 2 : NV == 2 && NT == 2 ? 3 : 4;         // what a thousand threads' share of shared memory holds
+  static constexpr int THREAD = KIND == kSingle ? 0 : AT * NT * NV * 16;       // bytes of shared memory
   uint8_t* ring;
-  typename P::Raw now[AHEAD ? 1 : NT][AHEAD ? 1 : NV];                         // elements by themselves: of the row that comes next
   __device__ __forceinline__ explicit Rows(uint8_t* shared) : ring(shared + threadIdx.x * 16) {}
   __device__ __forceinline__ uint8_t* slot(int stage, int tensor, int k) const { return ring + ((stage * NT + tensor) * NV + k) * (int)blockDim.x * 16; }
-  // tensors t of row `row`, columns of piece k from (mine + k * group) * VEC on
-  __device__ __forceinline__ void request(int stage, const T* const* from, bool there, int mine, int group, int width) {
-    if constexpr (AHEAD) {
+  // tensors' columns c0 + k * group * VEC ... of a row; `left`: elements from its first one to the tensor's end
+  __device__ __forceinline__ void request(int stage, const T* const* from, bool there, int c0, int group, int width, long long left) {
+    if constexpr (KIND != kSingle) {
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-          const int c = (mine + k * group) * VEC;
-          if (there && from[t] != nullptr && c < width)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(slot(stage, t, k))), "l"(from[t] + c) : "memory");
+          const int c = c0 + k * group * VEC;
+          if (there && from[t] != nullptr && c < width) {
+            const uint32_t to = (uint32_t)__cvta_generic_to_shared(slot(stage, t, k));
+            if (KIND == kShifted) {
+              const int bytes = left - c < VEC ? (int)(left - c) * (int)sizeof(T) : 16;
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from[t] + c), "r"(bytes) : "memory");
+            } else {
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from[t] + c) : "memory");
+            }
+          }
         }
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
   }
   __device__ __forceinline__ void arrived() const {
-    if constexpr (AHEAD) asm volatile("cp.async.wait_group %0;" ::"n"(AT - 1) : "memory");
-  }
-  // elements by themselves: the next row, once the current one has been read
-  __device__ __forceinline__ void fetch(const T* const* from, bool there, int mine, int group, int width) {
-    if constexpr (!AHEAD) {
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-          const int c = (mine + k * group) * VEC;
-          if (there && from[t] != nullptr && c < width) now[t][k] = P::load(from[t] + c);
-        }
-    }
+    if constexpr (KIND != kSingle) asm volatile("cp.async.wait_group %0;" ::"n"(AT - 1) : "memory");
   }
   __device__ __forceinline__ void all_arrived() const {
-    if constexpr (AHEAD) asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if constexpr (KIND != kSingle) asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
-  __device__ __forceinline__ void read(int stage, int tensor, int k, float* v) const {
-    if constexpr (AHEAD) P::unpack(*reinterpret_cast<const typename P::Raw*>(slot(stage, tensor, k)), v);
-    else P::unpack(now[tensor][k], v);
+  // columns c ... of the current row, zeros in those that are not the row's
+  __device__ __forceinline__ void read(int stage, int tensor, int k, const T* from, int c, int width, float* v) const {
+    if constexpr (KIND == kSingle) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[j] = c + j >= 0 && c + j < width ? to_f(from[c + j]) : 0.f;
+    } else {
+      P::unpack(*reinterpret_cast<const typename P::Raw*>(slot(stage, tensor, k)), v);
+      if (KIND == kShifted && (c < 0 || c + VEC > width)) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[j] = c + j >= 0 && c + j < width ? v[j] : 0.f;
+      }
+    }
+  }
+  // to rows one after the other, of which the first starts on 16 bytes
+  static __device__ __forceinline__ void write(T* to, int c, int width, const float* v) {
+    if (KIND == kAligned || (c >= 0 && c + VEC <= width)) {
+      P::store(to + c, v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (c + j >= 0 && c + j < width) to[c + j] = from_f<T>(v[j]);
+    }
   }
 };
 
@@ -184,57 +204,59 @@ __device__ __forceinline__ float2 group_all(float2 v, int group, float2 (*shared
   return v;
 }
 
-template <typename T, typename W, int VEC, int NV, bool QUANT>
+template <typename T, typename W, int VEC, int NV, int KIND, bool QUANT>
 __global__ void __launch_bounds__(512) norm_kernel(const NormRows p, T* __restrict__ y, uint8_t* __restrict__ codes, long long codes_ld, float* __restrict__ scales,
                                                     const int group) {
-  typedef Piece<T, VEC> P;
+  constexpr bool SHIFT = KIND != kAligned;
   extern __shared__ __align__(16) uint8_t ahead[];
   __shared__ float2 shared[2][16];
   pdl_sync();
   const int beside = blockDim.x / group, mine = threadIdx.x % group;
+  const long long step = (long long)gridDim.x * beside;
+  long long row = (long long)blockIdx.x * beside + threadIdx.x / group;
+  const int c0 = mine * VEC - (SHIFT ? (int)(row * p.width % VEC) : 0);        // this thread's first column
   const float inv_width = 1.0f / p.width;
   int turn = 0;
   float w[NV][VEC];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    const int c = (mine + k * group) * VEC;
+    const int c = c0 + k * group * VEC;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) w[k][j] = 1.0f;
-    if (p.weight != nullptr && c < p.width) load_weight<VEC>(static_cast<const W*>(p.weight) + c, w[k]);
+    if (p.weight != nullptr && c < p.width) load_weight<VEC, SHIFT>(static_cast<const W*>(p.weight), c, p.width, w[k]);
   }
-  Rows<T, VEC, NV, 2> rows(ahead);
-  constexpr int AT = rows.AT;
-  const long long step = (long long)gridDim.x * beside;
-  long long row = (long long)blockIdx.x * beside + threadIdx.x / group;
+  typedef Rows<T, VEC, NV, 2, KIND> R;
+  R rows(ahead);
+  constexpr int AT = R::AT;
   struct From { const T* at[2]; };
   auto from = [&](long long r) {
     return From{{static_cast<const T*>(p.x) + r * p.x_ld, p.res != nullptr ? static_cast<const T*>(p.res) + r * p.res_ld : nullptr}};
   };
-  auto request = [&](int stage, long long r) { rows.request(stage, from(r).at, r < p.rows, mine, group, p.width); };
+  auto request = [&](int stage, long long r) { rows.request(stage, from(r).at, r < p.rows, c0, group, p.width, (p.rows - r) * p.width); };
 #pragma unroll
   for (int k = 0; k < AT - 1; ++k) request(k, row + k * step);
-  rows.fetch(from(row).at, row < p.rows, mine, group, p.width);
   int stage = 0;
   // every thread goes as often as the block's first group: the sums synchronise
   for (long long base = (long long)blockIdx.x * beside; base < p.rows; base += step, row += step, stage = (stage + 1) % AT) {
     const bool there = row < p.rows;
     request((stage + AT - 1) % AT, row + (AT - 1) * step);
     rows.arrived();
+    const From at = from(row);
     float v[NV][VEC];
     float q = 0.f, most = 0.f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int c = (mine + k * group) * VEC;
+      const int c = c0 + k * group * VEC;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) v[k][j] = 0.f;
       if (there && c < p.width) {
-        rows.read(stage, 0, k, v[k]);
+        rows.read(stage, 0, k, at.at[0], c, p.width, v[k]);
         if (p.res != nullptr) {
           float r[VEC];
-          rows.read(stage, 1, k, r);
+          rows.read(stage, 1, k, at.at[1], c, p.width, r);
 #pragma unroll
           for (int j = 0; j < VEC; ++j) v[k][j] = to_f(from_f<T>(v[k][j] + r[j]));
-          P::store(static_cast<T*>(p.sum) + row * p.width + c, v[k]);
+          R::write(static_cast<T*>(p.sum) + row * p.width, c, p.width, v[k]);
         }
       }
 #pragma unroll
@@ -243,7 +265,6 @@ __global__ void __launch_bounds__(512) norm_kernel(const NormRows p, T* __restri
         if (QUANT) most = max_nan(most, fabsf(v[k][j] * w[k][j]));
       }
     }
-    rows.fetch(from(row + step).at, row + step < p.rows, mine, group, p.width);
     float rstd = 1.0f;
     if (QUANT || p.weight != nullptr) {
       const float2 r = group_all(make_float2(q, most), group, shared, turn, Add(), Max());
@@ -255,63 +276,65 @@ __global__ void __launch_bounds__(512) norm_kernel(const NormRows p, T* __restri
     if (QUANT && there && mine == 0) scales[row] = scale;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int c = (mine + k * group) * VEC;
+      const int c = c0 + k * group * VEC;
       const float factor = QUANT ? inv : rstd;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) v[k][j] = v[k][j] * factor * w[k][j];
       if (there && c < p.width) {
-        if (QUANT) store_codes<VEC>(codes + row * codes_ld + c, v[k]);
-        else P::store(y + row * p.width + c, v[k]);
+        if (QUANT) store_codes<VEC, SHIFT>(codes + row * codes_ld, c, p.width, v[k]);
+        else R::write(y + row * p.width, c, p.width, v[k]);
       }
     }
   }
 }
 
 // Gradients of rows and, in part[block], of the weight over the block's rows.
-template <typename T, typename W, int VEC, int NV>
+template <typename T, typename W, int VEC, int NV, int KIND>
 __global__ void __launch_bounds__(512, VEC * NV <= 8 ? 2 : 1) norm_bwd_kernel(const NormGrad p, const int group) {
-  typedef Piece<T, VEC> P;
+  constexpr bool SHIFT = KIND != kAligned;
   extern __shared__ __align__(16) uint8_t ahead[];
   __shared__ float2 shared[2][16];
   pdl_sync();
   const int beside = blockDim.x / group, mine = threadIdx.x % group;
+  const long long step = (long long)gridDim.x * beside;
+  long long row = (long long)blockIdx.x * beside + threadIdx.x / group;
+  const int c0 = mine * VEC - (SHIFT ? (int)(row * p.width % VEC) : 0);        // this thread's first column
   const float inv_width = 1.0f / p.width;
   int turn = 0;
   float w[NV][VEC], dw[NV][VEC];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    const int c = (mine + k * group) * VEC;
+    const int c = c0 + k * group * VEC;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) w[k][j] = dw[k][j] = 0.f;
-    if (c < p.width) load_weight<VEC>(static_cast<const W*>(p.weight) + c, w[k]);
+    if (c < p.width) load_weight<VEC, SHIFT>(static_cast<const W*>(p.weight), c, p.width, w[k]);
   }
-  Rows<T, VEC, NV, 3> rows(ahead);
-  constexpr int AT = rows.AT;
-  const long long step = (long long)gridDim.x * beside;
-  long long row = (long long)blockIdx.x * beside + threadIdx.x / group;
+  typedef Rows<T, VEC, NV, 3, KIND> R;
+  R rows(ahead);
+  constexpr int AT = R::AT;
   struct From { const T* at[3]; };
   auto from = [&](long long r) {
     return From{{static_cast<const T*>(p.s) + r * p.s_ld, static_cast<const T*>(p.dy) + r * p.dy_ld, p.ds != nullptr ? static_cast<const T*>(p.ds) + r * p.ds_ld : nullptr}};
   };
-  auto request = [&](int stage, long long r) { rows.request(stage, from(r).at, r < p.rows, mine, group, p.width); };
+  auto request = [&](int stage, long long r) { rows.request(stage, from(r).at, r < p.rows, c0, group, p.width, (p.rows - r) * p.width); };
 #pragma unroll
   for (int k = 0; k < AT - 1; ++k) request(k, row + k * step);
-  rows.fetch(from(row).at, row < p.rows, mine, group, p.width);
   int stage = 0;
   for (long long base = (long long)blockIdx.x * beside; base < p.rows; base += step, row += step, stage = (stage + 1) % AT) {
     const bool there = row < p.rows;
     request((stage + AT - 1) % AT, row + (AT - 1) * step);
     rows.arrived();
+    const From at = from(row);
     float s[NV][VEC], g[NV][VEC];
     float q = 0.f, d = 0.f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int c = (mine + k * group) * VEC;
+      const int c = c0 + k * group * VEC;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) s[k][j] = g[k][j] = 0.f;
       if (there && c < p.width) {
-        rows.read(stage, 0, k, s[k]);
-        rows.read(stage, 1, k, g[k]);
+        rows.read(stage, 0, k, at.at[0], c, p.width, s[k]);
+        rows.read(stage, 1, k, at.at[1], c, p.width, g[k]);
       }
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
@@ -319,31 +342,22 @@ __global__ void __launch_bounds__(512, VEC * NV <= 8 ? 2 : 1) norm_bwd_kernel(co
         d = fmaf(s[k][j] * g[k][j], w[k][j], d);
       }
     }
-    typename P::Raw add[rows.AHEAD ? 1 : NV];
-    if constexpr (!rows.AHEAD) {
-#pragma unroll
-      for (int k = 0; k < NV; ++k) add[k] = rows.now[2][k];
-      rows.fetch(from(row + step).at, row + step < p.rows, mine, group, p.width);
-    }
     const float2 r = group_all(make_float2(q, d), group, shared, turn, Add(), Add());
     const float rstd = rsqrtf(r.x * inv_width + p.eps), along = r.y * rstd * inv_width * rstd;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int c = (mine + k * group) * VEC;
+      const int c = c0 + k * group * VEC;
       float o[VEC];
 #pragma unroll
       for (int j = 0; j < VEC; ++j) o[j] = 0.f;
-      if (p.ds != nullptr && there && c < p.width) {
-        if constexpr (rows.AHEAD) rows.read(stage, 2, k, o);
-        else P::unpack(add[k], o);
-      }
+      if (p.ds != nullptr && there && c < p.width) rows.read(stage, 2, k, at.at[2], c, p.width, o);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         const float n = s[k][j] * rstd;
         dw[k][j] = fmaf(g[k][j], n, dw[k][j]);
         o[j] = fmaf(g[k][j] * w[k][j], rstd, fmaf(-n, along, o[j]));
       }
-      if (there && c < p.width) P::store(static_cast<T*>(p.dx) + row * p.width + c, o);
+      if (there && c < p.width) R::write(static_cast<T*>(p.dx) + row * p.width, c, p.width, o);
     }
   }
   float* part = p.part + (long long)blockIdx.x * p.width;
@@ -351,20 +365,22 @@ __global__ void __launch_bounds__(512, VEC * NV <= 8 ? 2 : 1) norm_bwd_kernel(co
   if (beside == 1) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int c = (mine + k * group) * VEC;
+      const int c = c0 + k * group * VEC;
       if (c < p.width)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) part[c + j] = dw[k][j];
+        for (int j = 0; j < VEC; ++j)
+          if (!SHIFT || (c + j >= 0 && c + j < p.width)) part[c + j] = dw[k][j];
     }
   } else {
     float* sums = reinterpret_cast<float*>(ahead);         // [group][width], where the rows were
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int c = (mine + k * group) * VEC;
+      const int c = c0 + k * group * VEC;
       if (c < p.width)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) sums[threadIdx.x / group * p.width + c + j] = dw[k][j];
+        for (int j = 0; j < VEC; ++j)
+          if (!SHIFT || (c + j >= 0 && c + j < p.width)) sums[threadIdx.x / group * p.width + c + j] = dw[k][j];
     }
     __syncthreads();
     for (int c = threadIdx.x; c < p.width; c += blockDim.x) {
@@ -478,14 +494,14 @@ __global__ void __launch_bounds__(kThreads) wide_norm_dw_kernel(const NormGrad p
 // How many pieces a thread holds and how many threads share a row: two pieces each where the rows alone fill the SMs (fewer threads to
 // join for each sum), one where a row's latency counts.
 struct Layout { int pieces, group; };       // pieces 0: the row does not fit
-Layout layout_of(long long rows, int width, int vec, int most_pieces) {
-  const int all = (width + vec - 1) / vec;
+Layout layout_of(long long rows, int width, int vec) {
+  const int all = width % vec == 0 ? width / vec : (width + 2 * vec - 2) / vec, most_pieces = 4;
   auto group_for = [&](int pieces) {
     int g = 32;
     while (g < 512 && g * pieces < all) g *= 2;
     return g;
   };
-  int pieces = vec == 1 ? 4 : rows >= 4LL * sm_count() ? 2 : 1;
+  int pieces = rows >= 4LL * sm_count() ? 2 : 1;
   while (pieces < most_pieces && group_for(pieces) * pieces < all) pieces *= 2;
   const int group = group_for(pieces);
   return group * pieces < all ? Layout{0, 0} : Layout{pieces, group};
@@ -493,14 +509,27 @@ Layout layout_of(long long rows, int width, int vec, int most_pieces) {
 int block_of(int group) { return group < 256 ? 256 : group; }
 
 bool aligned(const void* p, long long ld, int bytes) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * bytes % 16 == 0; }
-bool in_pieces(const NormRows& p) {
+Kind kind_of(const NormRows& p, const void* y) {
   const int size = p.bf16 ? 2 : 4;
-  return aligned(p.x, p.x_ld, size) && aligned(p.res, p.res_ld, size) && aligned(p.sum, p.width, size) && aligned(p.weight, 0, 1) && p.width * size % 16 == 0;
+  auto fits = [&](int bytes) {
+    return aligned(p.x, p.x_ld, bytes) && aligned(p.res, p.res_ld, bytes) && aligned(p.sum, p.width, bytes) && aligned(y, p.width, bytes);
+  };
+  if (fits(size) && p.width * size % 16 == 0 && aligned(p.weight, 0, 1)) return kAligned;
+  return fits(16) && p.x_ld == p.width && (p.res == nullptr || p.res_ld == p.width) ? kShifted : kSingle;
 }
-bool in_pieces(const NormGrad& p) {
+Kind kind_of(const NormGrad& p) {
   const int size = p.bf16 ? 2 : 4;
-  return aligned(p.s, p.s_ld, size) && aligned(p.dy, p.dy_ld, size) && aligned(p.ds, p.ds_ld, size) && aligned(p.dx, p.width, size) && aligned(p.weight, 0, 1) &&
-         p.width * size % 16 == 0;
+  auto fits = [&](int bytes) {
+    return aligned(p.s, p.s_ld, bytes) && aligned(p.dy, p.dy_ld, bytes) && aligned(p.ds, p.ds_ld, bytes) && aligned(p.dx, p.width, bytes);
+  };
+  if (fits(size) && p.width * size % 16 == 0 && aligned(p.weight, 0, 1)) return kAligned;
+  return fits(16) && p.s_ld == p.width && p.dy_ld == p.width && (p.ds == nullptr || p.ds_ld == p.width) ? kShifted : kSingle;
+}
+// Blocks whose groups walk along rows that are shifted alike.
+long long walking(long long blocks, long long most, int beside, int vec) {
+  if (blocks <= most) return blocks;
+  while (most > 1 && most * beside % vec != 0) --most;
+  return most;
 }
 
 // More shared memory than a kernel has by itself has to be asked for, once.
@@ -515,34 +544,31 @@ cudaError_t allow(const void* kernel, size_t smem) {
   return e;
 }
 
-template <typename T, typename W, bool QUANT, int VEC>
+template <typename T, typename W, bool QUANT, int KIND>
 cudaError_t forward_rows(const NormRows& p, const Layout& l, void* y, void* codes, long long codes_ld, float* scales, cudaStream_t st) {
+  constexpr int VEC = 16 / sizeof(T);
   const int block = block_of(l.group), beside = block / l.group;
-  const long long blocks = (p.rows + beside - 1) / beside, most = (long long)sm_count() * (l.pieces * VEC <= 8 ? 2048 : 768) / block;
+  const long long blocks = walking((p.rows + beside - 1) / beside, (long long)sm_count() * (l.pieces * VEC <= 8 ? 2048 : 1024) / block, beside, VEC);
   auto with = [&](auto kernel, int thread) {
     const size_t smem = (size_t)thread * block;
     const cudaError_t e = allow(reinterpret_cast<const void*>(kernel), smem);
     if (e != cudaSuccess) return e;
-    return launch_pdl(kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(block), smem, st, p, static_cast<T*>(y), static_cast<uint8_t*>(codes), codes_ld, scales,
-                      l.group);
+    return launch_pdl(kernel, dim3((unsigned)blocks), dim3(block), smem, st, p, static_cast<T*>(y), static_cast<uint8_t*>(codes), codes_ld, scales, l.group);
   };
-  if constexpr (VEC > 1) {
-    if (l.pieces == 1) return with(norm_kernel<T, W, VEC, 1, QUANT>, Rows<T, VEC, 1, 2>::THREAD);
-    if (l.pieces == 2) return with(norm_kernel<T, W, VEC, 2, QUANT>, Rows<T, VEC, 2, 2>::THREAD);
-    return with(norm_kernel<T, W, VEC, 4, QUANT>, Rows<T, VEC, 4, 2>::THREAD);
-  } else {
-    if (l.pieces == 4) return with(norm_kernel<T, W, VEC, 4, QUANT>, Rows<T, VEC, 4, 2>::THREAD);
-    return l.pieces == 8 ? with(norm_kernel<T, W, VEC, 8, QUANT>, Rows<T, VEC, 8, 2>::THREAD) : with(norm_kernel<T, W, VEC, 16, QUANT>, Rows<T, VEC, 16, 2>::THREAD);
-  }
+  if (l.pieces == 1) return with(norm_kernel<T, W, VEC, 1, KIND, QUANT>, Rows<T, VEC, 1, 2, KIND>::THREAD);
+  if (l.pieces == 2) return with(norm_kernel<T, W, VEC, 2, KIND, QUANT>, Rows<T, VEC, 2, 2, KIND>::THREAD);
+  return with(norm_kernel<T, W, VEC, 4, KIND, QUANT>, Rows<T, VEC, 4, 2, KIND>::THREAD);
 }
 template <typename T, typename W, bool QUANT>
 cudaError_t forward(const NormRows& p, void* y, void* codes, long long codes_ld, float* scales, cudaStream_t st) {
   if (p.rows <= 0) return cudaSuccess;
-  constexpr int VEC = 16 / sizeof(T);
-  const bool pieces = in_pieces(p) && aligned(y, p.width, sizeof(T));
-  const Layout l = layout_of(p.rows, p.width, pieces ? VEC : 1, pieces ? 4 : 16);
-  if (l.pieces != 0)
-    return pieces ? forward_rows<T, W, QUANT, VEC>(p, l, y, codes, codes_ld, scales, st) : forward_rows<T, W, QUANT, 1>(p, l, y, codes, codes_ld, scales, st);
+  const Kind kind = kind_of(p, y);
+  const Layout l = layout_of(p.rows, p.width, 16 / sizeof(T));
+  if (l.pieces != 0) {
+    if (kind == kAligned) return forward_rows<T, W, QUANT, kAligned>(p, l, y, codes, codes_ld, scales, st);
+    if (kind == kShifted) return forward_rows<T, W, QUANT, kShifted>(p, l, y, codes, codes_ld, scales, st);
+    return forward_rows<T, W, QUANT, kSingle>(p, l, y, codes, codes_ld, scales, st);
+  }
   const long long most = 8LL * sm_count();
   return launch_pdl(wide_norm_kernel<T, W, QUANT>, dim3((unsigned)(p.rows < most ? p.rows : most)), dim3(kThreads), 0, st, p, static_cast<T*>(y),
                     static_cast<uint8_t*>(codes), codes_ld, scales);
@@ -556,44 +582,40 @@ cudaError_t forward_of(const NormRows& p, void* y, void* codes, long long codes_
 constexpr int kWideParts = 64;
 constexpr int kThreadsBack = 512;            // on an SM, twice as many where a thread has 8 columns at most
 
-Layout layout_back(const NormGrad& p) {
-  const bool pieces = in_pieces(p);
-  return layout_of(pieces ? p.rows : 0, p.width, pieces ? (p.bf16 ? 8 : 4) : 1, pieces ? 4 : 16);
-}
-int blocks_back(const NormGrad& p, const Layout& l) {
-  const int beside = block_of(l.group) / l.group;
-  const long long blocks = (p.rows + beside - 1) / beside, most = (long long)sm_count() * (kThreadsBack / block_of(l.group)) * (l.pieces * (in_pieces(p) ? (p.bf16 ? 8 : 4) : 1) <= 8 ? 2 : 1);
-  return (int)(blocks < most ? blocks : most);
+Layout layout_back(const NormGrad& p) { return layout_of(p.rows, p.width, p.bf16 ? 8 : 4); }
+long long blocks_back(const NormGrad& p, const Layout& l) {
+  const int block = block_of(l.group), beside = block / l.group, vec = p.bf16 ? 8 : 4;
+  const long long most = (long long)sm_count() * (kThreadsBack / block) * (l.pieces * vec <= 8 ? 2 : 1);
+  return walking((p.rows + beside - 1) / beside, most, beside, vec);
 }
 
-template <typename T, typename W, int VEC>
+template <typename T, typename W, int KIND>
 cudaError_t backward_rows(const NormGrad& p, const Layout& l, cudaStream_t st) {
+  constexpr int VEC = 16 / sizeof(T);
   const int block = block_of(l.group), beside = block / l.group;
   auto with = [&](auto kernel, int thread) {
     const size_t joined = beside > 1 ? (size_t)beside * p.width * sizeof(float) : 0, ahead = (size_t)thread * block, smem = joined > ahead ? joined : ahead;
     const cudaError_t e = allow(reinterpret_cast<const void*>(kernel), smem);
     if (e != cudaSuccess) return e;
-    return launch_pdl(kernel, dim3(blocks_back(p, l)), dim3(block), smem, st, p, l.group);
+    return launch_pdl(kernel, dim3((unsigned)blocks_back(p, l)), dim3(block), smem, st, p, l.group);
   };
-  if constexpr (VEC > 1) {
-    if (l.pieces == 1) return with(norm_bwd_kernel<T, W, VEC, 1>, Rows<T, VEC, 1, 3>::THREAD);
-    if (l.pieces == 2) return with(norm_bwd_kernel<T, W, VEC, 2>, Rows<T, VEC, 2, 3>::THREAD);
-    return with(norm_bwd_kernel<T, W, VEC, 4>, Rows<T, VEC, 4, 3>::THREAD);
-  } else {
-    if (l.pieces == 4) return with(norm_bwd_kernel<T, W, VEC, 4>, Rows<T, VEC, 4, 3>::THREAD);
-    return l.pieces == 8 ? with(norm_bwd_kernel<T, W, VEC, 8>, Rows<T, VEC, 8, 3>::THREAD) : with(norm_bwd_kernel<T, W, VEC, 16>, Rows<T, VEC, 16, 3>::THREAD);
-  }
+  if (l.pieces == 1) return with(norm_bwd_kernel<T, W, VEC, 1, KIND>, Rows<T, VEC, 1, 3, KIND>::THREAD);
+  if (l.pieces == 2) return with(norm_bwd_kernel<T, W, VEC, 2, KIND>, Rows<T, VEC, 2, 3, KIND>::THREAD);
+  return with(norm_bwd_kernel<T, W, VEC, 4, KIND>, Rows<T, VEC, 4, 3, KIND>::THREAD);
 }
 template <typename T, typename W>
 cudaError_t backward(const NormGrad& p, int* launched, cudaStream_t st) {
+  const Kind kind = kind_of(p);
   const Layout l = layout_back(p);
   int parts = 0;
   cudaError_t e = cudaSuccess;
   *launched = 1;
   if (p.rows > 0 && l.pieces != 0) {
-    parts = blocks_back(p, l);
+    parts = (int)blocks_back(p, l);
     *launched = 2;
-    e = in_pieces(p) ? backward_rows<T, W, 16 / sizeof(T)>(p, l, st) : backward_rows<T, W, 1>(p, l, st);
+    if (kind == kAligned) e = backward_rows<T, W, kAligned>(p, l, st);
+    else if (kind == kShifted) e = backward_rows<T, W, kShifted>(p, l, st);
+    else e = backward_rows<T, W, kSingle>(p, l, st);
   } else if (p.rows > 0) {
     parts = kWideParts;
     *launched = 3;
@@ -615,7 +637,7 @@ cudaError_t rms_norm_8bit(const NormRows& p, void* codes, long long codes_ld, fl
 }
 long long rms_norm_bwd_floats(const NormGrad& p) {
   const Layout l = layout_back(p);
-  return l.pieces != 0 ? (long long)blocks_back(p, l) * p.width : (long long)kWideParts * p.width + p.rows;       // the rows' rstd behind the sums
+  return l.pieces != 0 ? blocks_back(p, l) * p.width : (long long)kWideParts * p.width + p.rows;       // the rows' rstd behind the sums
 }
 cudaError_t rms_norm_bwd(const NormGrad& p, int* launched, cudaStream_t st) {
   if (!p.bf16) return p.weight_bf16 ? cudaErrorInvalidValue : backward<float, float>(p, launched, st);
