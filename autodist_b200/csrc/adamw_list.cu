@@ -13,20 +13,25 @@
 #include <cuda_fp8.h>
 
 #include "pdl.cuh"
+#include "sm_count.h"
 
 namespace adb200 {
 namespace {
 
 typedef __nv_bfloat16 bf16;
 constexpr int kThreads = 256;
+constexpr int kChunk = 4096;                             // elements of a tensor that a thread block updates at a time
+constexpr int kBlocks8 = 4, kBlocks32 = 4;               // on an SM
 constexpr float kE4m3Max = 448.0f;
-constexpr float kTiniest = 7.888609052210118e-31f;        // 2^-100: blocks below are held as zeros, their scale's inverse would overflow
-static_assert(sizeof(AdamwTable) + 256 <= 32764, "kernel parameters");
+constexpr float kTiniest = 7.888609052210118e-31f;       // 2^-100: blocks below are held as zeros, their scale's inverse would overflow
 
-__device__ __forceinline__ float to_f(float v) { return v; }
-__device__ __forceinline__ float to_f(bf16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ void put(float* p, float v) { *p = v; }
-__device__ __forceinline__ void put(bf16* p, float v) { *p = __float2bfloat16(v); }
+// A launch copies its parameters: few tensors travel in a small table.
+template <int MOST> struct Table {
+  int count;
+  int first[MOST + 1];                                   // chunks of the tensors in front
+  AdamwTensor t[MOST];
+};
+static_assert(sizeof(Table<kAdamwMost>) + 256 <= 32764, "kernel parameters");
 
 // 64 mixed bits of a counter, as the dropout decisions use them
 __device__ __forceinline__ uint64_t mixed(uint64_t seed, uint64_t i) {
@@ -42,19 +47,25 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// The e4m3 value at |v| <= 448 (and a rounding), rounded up where the cut-off part and the random 16 bits add up to one.
-__device__ __forceinline__ uint8_t round_random(float v, uint32_t bits16) {
+// The e4m3 code of v (|v| <= 448, or a rounding more), rounded up where the cut-off part and u = (bits16 + 1/2) / 65536 add up to one. Codes are
+// a float's sign, exponent and upper three bits of the fraction: u is added below those, and what carries over is the rounding. Sizes
+// below 2^-6, whose codes are multiples of 2^-9, are moved up by 2^-6 first, where the steps are the same.
+__device__ __forceinline__ uint32_t round_random(float v, uint32_t bits16) {
   const float size = fabsf(v);
-  const uint32_t binade = __float_as_uint(fmaxf(size, 0.015625f)) & 0x7F800000u;       // the power of two below, 2^-6 for the smallest
-  const float ulp = __uint_as_float(binade - (3u << 23)), inv = __uint_as_float((254u << 23) - (binade - (3u << 23)));
-  const float u = ((float)bits16 + 0.5f) * (1.0f / 65536.0f);
-  float q = floorf(__fadd_rn(__fmul_rn(size, inv), u)) * ulp;
-  if (q > kE4m3Max) q = kE4m3Max;
-  if (q == 0.f && size > 0.f) q = 0.001953125f;
-  return __nv_cvt_float_to_fp8(copysignf(q, v), __NV_SATFINITE, __NV_E4M3);
+  const bool small = size < 0.015625f;
+  const uint32_t at = __float_as_uint(small ? __fadd_rz(size, 0.015625f) : size) + (bits16 << 4) + 8u;
+  uint32_t code = (at >> 20) - (small ? 968u : 960u);
+  code = min(code, 126u);                                // 448
+  if (code == 0u && size > 0.f) code = 1u;
+  if (size != size) code = 127u;
+  return code | (__float_as_uint(v) >> 24 & 0x80u);
 }
 
-__device__ __forceinline__ float of_e4m3(uint8_t c) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3))); }
+// Two e4m3 codes of a word's lower half
+__device__ __forceinline__ float2 of_e4m3x2(uint32_t codes) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)codes, __NV_E4M3);
+  return __half22float2(__half2(h));
+}
 
 struct Step {
   float decay, rate, spread, b1, c1, b2, c2, eps;
@@ -77,80 +88,131 @@ __device__ __forceinline__ void update(const Step& s, float& p, float g, float& 
   m = __fadd_rn(__fmul_rn(s.b1, m), __fmul_rn(s.c1, g));
   v = __fadd_rn(__fmul_rn(s.b2, v), __fmul_rn(s.c2, __fmul_rn(g, g)));
   root = __fsqrt_rn(v);
-  p = p * s.decay - s.rate * (m / (root * s.spread + s.eps));
+  p = fmaf(p, s.decay, -s.rate * __fdividef(m, fmaf(root, s.spread, s.eps)));
 }
 
-// A thread block per chunk of a tensor; a warp's blocks of 256 elements one after the other.
-template <typename P, typename G, bool BITS8>
-__global__ void __launch_bounds__(kThreads) adamw_list_kernel(const __grid_constant__ AdamwTable table, const AdamwMoments mo, const AdamwRule rule) {
-  pdl_sync();
+// Eight neighbouring elements, of which `n` are there (8 or more: all, on 16 bytes).
+__device__ __forceinline__ void load8(const float* p, int n, bool whole, float* v) {
+  if (whole) {
+    const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < n ? p[j] : 0.f;
+  }
+}
+__device__ __forceinline__ void load8(const bf16* p, int n, bool whole, float* v) {
+  if (whole) {
+    const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p));
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { v[2 * j] = __uint_as_float(w[j] << 16); v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u); }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < n ? __bfloat162float(p[j]) : 0.f;
+  }
+}
+__device__ __forceinline__ void store8(float* p, int n, bool whole, const float* v) {
+  if (whole) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) if (j < n) p[j] = v[j];
+  }
+}
+__device__ __forceinline__ void store8(bf16* p, int n, bool whole, const float* v) {
+  if (whole) {
+    uint4 a;
+    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&a);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h[j] = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+    *reinterpret_cast<uint4*>(p) = a;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) if (j < n) p[j] = __float2bfloat16(v[j]);
+  }
+}
+
+// A warp updates 256 elements at a time, a lane eight neighbours of them, so that the largest moments are found in registers and every byte
+// moves once. Blocks walk along the list's chunks: what a step's elements share (two powers in double) is computed once for each.
+template <typename P, typename G, bool BITS8, int MOST>
+__global__ void __launch_bounds__(kThreads) adamw_list_kernel(const __grid_constant__ Table<MOST> table, const AdamwMoments mo, const AdamwRule rule) {
   __shared__ Step shared;
+  pdl_sync();
   if (threadIdx.x == 0) shared = step_of(rule, rule.step[0] + 1);
   __syncthreads();
   const Step s = shared;
-  const int chunk = blockIdx.x;
-  int lo = 0, hi = table.count;              // the tensor whose chunk this is
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (table.first[mid] <= chunk) lo = mid; else hi = mid;
-  }
-  const AdamwTensor t = table.t[lo];
-  const long long start = (long long)(chunk - table.first[lo]) * kAdamwChunk;
-  const int lane = threadIdx.x & 31;
-  for (int k = (threadIdx.x >> 5) * kAdamwBlock; k < kAdamwChunk && start + k < t.n; k += kThreads / 32 * kAdamwBlock) {
-    const long long place = t.place + start + k;
-    float m[8], root[8];
-    float m_most = 0.f, r_most = 0.f;
-    const float m_scale = BITS8 ? mo.m_scale[place / kAdamwBlock] : 0.f, r_scale = BITS8 ? mo.r_scale[place / kAdamwBlock] : 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const long long i = start + k + 32 * j + lane;
-      const long long q = place + 32 * j + lane;
-      m[j] = root[j] = 0.f;
-      if (i < t.n) {
-        float v;
-        if (BITS8) {
-          m[j] = __fmul_rn(of_e4m3(static_cast<const uint8_t*>(mo.m)[q]), m_scale);
-          v = __fmul_rn(of_e4m3(static_cast<const uint8_t*>(mo.r)[q]), r_scale);
-          v = __fmul_rn(v, v);
-        } else {
-          m[j] = static_cast<const float*>(mo.m)[q];
-          v = static_cast<const float*>(mo.r)[q];
-        }
-        P* pp = static_cast<P*>(t.p) + i;
-        float p = to_f(*pp);
-        update(s, p, to_f(static_cast<const G*>(t.g)[i]), m[j], v, root[j]);
-        put(pp, p);
-        if (!BITS8) {
-          static_cast<float*>(mo.m)[q] = m[j];
-          static_cast<float*>(mo.r)[q] = v;
-        }
-        m_most = max_nan(m_most, fabsf(m[j]));
-        r_most = max_nan(r_most, root[j]);
-      }
+  const int lane = threadIdx.x & 31, chunks = table.first[table.count];
+  for (int chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+    int lo = 0, hi = table.count;              // the tensor whose chunk this is
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (table.first[mid] <= chunk) lo = mid; else hi = mid;
     }
-    if (BITS8) {
+    const AdamwTensor& t = table.t[lo];
+    P* const params = static_cast<P*>(t.p);
+    const G* const grads = static_cast<const G*>(t.g);
+    const long long size = t.n, start = (long long)(chunk - table.first[lo]) * kChunk;
+    const bool vectors = ((reinterpret_cast<uintptr_t>(params) | reinterpret_cast<uintptr_t>(grads)) & 15) == 0;
+    for (int k = (threadIdx.x >> 5) * kAdamwBlock; k < kChunk && start + k < size; k += kThreads / 32 * kAdamwBlock) {
+      const long long i = start + k + 8 * lane, q = t.place + i, block = (t.place + start + k) / kAdamwBlock;
+      const int n = size - i > 8 ? 8 : (int)(size - i);  // of this lane's elements, can be none
+      const bool whole = vectors && n == 8;
+      float p[8], g[8], m[8], v[8], root[8];
+      load8(params + i, n, whole, p);
+      load8(grads + i, n, whole, g);
+      if (BITS8) {                                       // moments are padded to whole blocks
+        const uint2 mc = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(mo.m) + q)), rc = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(mo.r) + q));
+        const float m_scale = mo.m_scale[block], r_scale = mo.r_scale[block];
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        m_most = max_nan(m_most, __shfl_xor_sync(0xffffffffu, m_most, o));
-        r_most = max_nan(r_most, __shfl_xor_sync(0xffffffffu, r_most, o));
+        for (int j = 0; j < 4; ++j) {
+          const float2 a = of_e4m3x2((j < 2 ? mc.x : mc.y) >> (16 * (j & 1)) & 0xFFFFu), b = of_e4m3x2((j < 2 ? rc.x : rc.y) >> (16 * (j & 1)) & 0xFFFFu);
+          m[2 * j] = __fmul_rn(a.x, m_scale); m[2 * j + 1] = __fmul_rn(a.y, m_scale);
+          v[2 * j] = __fmul_rn(b.x, r_scale); v[2 * j + 1] = __fmul_rn(b.y, r_scale);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(v[j], v[j]);
+      } else {
+        load8(static_cast<const float*>(mo.m) + q, 8, true, m);
+        load8(static_cast<const float*>(mo.r) + q, 8, true, v);
       }
-      const bool m_held = !(m_most < kTiniest), r_held = !(r_most < kTiniest);
-      const float m_inv = m_held ? __fmul_rn(__frcp_rn(m_most), kE4m3Max) : 0.f, r_inv = r_held ? __fmul_rn(__frcp_rn(r_most), kE4m3Max) : 0.f;
+      float m_most = 0.f, r_most = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const long long i = start + k + 32 * j + lane;
-        const long long q = place + 32 * j + lane;
-        if (i < t.n) {
-          const uint64_t word = mixed(s.key, (uint64_t)q >> 1);
-          const uint32_t bits = (uint32_t)(word >> ((q & 1) * 32));
-          static_cast<uint8_t*>(mo.m)[q] = round_random(__fmul_rn(m[j], m_inv), bits & 0xFFFFu);
-          static_cast<uint8_t*>(mo.r)[q] = round_random(__fmul_rn(root[j], r_inv), bits >> 16);
+        update(s, p[j], g[j], m[j], v[j], root[j]);
+        if (BITS8 && j < n) {
+          m_most = max_nan(m_most, fabsf(m[j]));
+          r_most = max_nan(r_most, root[j]);
         }
       }
-      if (lane == 0) {
-        mo.m_scale[place / kAdamwBlock] = m_held ? __fmul_rn(m_most, 1.0f / kE4m3Max) : 0.f;
-        mo.r_scale[place / kAdamwBlock] = r_held ? __fmul_rn(r_most, 1.0f / kE4m3Max) : 0.f;
+      store8(params + i, n, whole, p);
+      if (BITS8) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          m_most = max_nan(m_most, __shfl_xor_sync(0xffffffffu, m_most, o));
+          r_most = max_nan(r_most, __shfl_xor_sync(0xffffffffu, r_most, o));
+        }
+        const bool m_held = !(m_most < kTiniest), r_held = !(r_most < kTiniest);
+        const float m_inv = m_held ? __fmul_rn(__frcp_rn(m_most), kE4m3Max) : 0.f, r_inv = r_held ? __fmul_rn(__frcp_rn(r_most), kE4m3Max) : 0.f;
+        uint32_t mc[2] = {0u, 0u}, rc[2] = {0u, 0u};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint64_t word = mixed(s.key, (uint64_t)(q + j) >> 1);          // shared by two neighbours
+          const uint32_t bits = (uint32_t)(word >> (32 * (j & 1)));
+          const bool there = j < n;
+          mc[j >> 2] |= (there ? round_random(__fmul_rn(m[j], m_inv), bits & 0xFFFFu) : 0u) << (8 * (j & 3));
+          rc[j >> 2] |= (there ? round_random(__fmul_rn(root[j], r_inv), bits >> 16) : 0u) << (8 * (j & 3));
+        }
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(mo.m) + q) = make_uint2(mc[0], mc[1]);
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(mo.r) + q) = make_uint2(rc[0], rc[1]);
+        if (lane == 0) {
+          mo.m_scale[block] = m_held ? __fmul_rn(m_most, 1.0f / kE4m3Max) : 0.f;
+          mo.r_scale[block] = r_held ? __fmul_rn(r_most, 1.0f / kE4m3Max) : 0.f;
+        }
+      } else {
+        store8(static_cast<float*>(mo.m) + q, n, n == 8, m);
+        store8(static_cast<float*>(mo.r) + q, n, n == 8, v);
       }
     }
   }
@@ -164,18 +226,33 @@ __global__ void __launch_bounds__(kThreads) adamw_list_kernel(const __grid_const
   }
 }
 
+template <typename P, typename G, int MOST>
+cudaError_t step_of_list(const AdamwTensor* tensors, int count, const AdamwMoments& mo, const AdamwRule& rule, cudaStream_t st) {
+  Table<MOST> table;
+  table.count = count;
+  long long chunks = 0;
+  for (int i = 0; i < count; ++i) {
+    table.first[i] = (int)chunks;
+    table.t[i] = tensors[i];
+    chunks += (tensors[i].n + kChunk - 1) / kChunk;
+    if (chunks > 0x7fffffffLL) return cudaErrorInvalidValue;
+  }
+  table.first[count] = (int)chunks;
+  const long long most = (long long)sm_count() * (mo.m_scale != nullptr ? kBlocks8 : kBlocks32);
+  return launch_pdl(mo.m_scale != nullptr ? adamw_list_kernel<P, G, true, MOST> : adamw_list_kernel<P, G, false, MOST>, dim3((unsigned)(chunks < most ? chunks : most)),
+                    dim3(kThreads), 0, st, table, mo, rule);
+}
 template <typename P, typename G>
-cudaError_t step_of_types(const AdamwTable& table, const AdamwMoments& mo, const AdamwRule& rule, cudaStream_t st) {
-  const dim3 grid((unsigned)table.first[table.count]);
-  return launch_pdl(mo.m_scale != nullptr ? adamw_list_kernel<P, G, true> : adamw_list_kernel<P, G, false>, grid, dim3(kThreads), 0, st, table, mo, rule);
+cudaError_t step_of_types(const AdamwTensor* tensors, int count, const AdamwMoments& mo, const AdamwRule& rule, cudaStream_t st) {
+  return count <= 96 ? step_of_list<P, G, 96>(tensors, count, mo, rule, st) : step_of_list<P, G, kAdamwMost>(tensors, count, mo, rule, st);
 }
 
 }  // namespace
 
-cudaError_t adamw_list_step(const AdamwTable& table, bool p_bf16, bool g_bf16, const AdamwMoments& mo, const AdamwRule& rule, cudaStream_t st) {
-  if (table.count <= 0 || table.first[table.count] <= 0) return cudaErrorInvalidValue;
-  if (p_bf16) return g_bf16 ? step_of_types<bf16, bf16>(table, mo, rule, st) : step_of_types<bf16, float>(table, mo, rule, st);
-  return g_bf16 ? step_of_types<float, bf16>(table, mo, rule, st) : step_of_types<float, float>(table, mo, rule, st);
+cudaError_t adamw_list_step(const AdamwTensor* tensors, int count, bool p_bf16, bool g_bf16, const AdamwMoments& mo, const AdamwRule& rule, cudaStream_t st) {
+  if (count <= 0 || count > kAdamwMost) return cudaErrorInvalidValue;
+  if (p_bf16) return g_bf16 ? step_of_types<bf16, bf16>(tensors, count, mo, rule, st) : step_of_types<bf16, float>(tensors, count, mo, rule, st);
+  return g_bf16 ? step_of_types<float, bf16>(tensors, count, mo, rule, st) : step_of_types<float, float>(tensors, count, mo, rule, st);
 }
 
 }  // namespace adb200

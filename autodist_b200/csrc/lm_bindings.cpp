@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <atomic>
 #include <memory>
 #include <string>
@@ -442,13 +443,13 @@ int64_t adamw_list_step(const std::shared_ptr<AdamwList>& l, double lr, const op
   const c10::cuda::CUDAGuard guard(first.device());
   const cudaStream_t st = stream_of(first);
   if (lr_at.has_value()) TORCH_CHECK(same_gpu(first, *lr_at) && lr_at->scalar_type() == at::kFloat && lr_at->numel() == 1, "adamw: an fp32 learning rate on the GPU needed");
-  struct Batch { bool p16, g16; std::unique_ptr<adb200::AdamwTable> table; };
+  struct Batch { bool p16, g16; std::vector<adb200::AdamwTensor> tensors; };
   std::vector<Batch> batches;
   std::vector<Tensor> held;                                  // gradients and parameters that had to be laid out
   std::vector<std::pair<Tensor, Tensor>> back;               // parameters to copy into, from their laid-out copies
   for (size_t i = 0; i < l->params.size(); ++i) {
+    if (!l->params[i].grad().defined() || l->params[i].numel() == 0) continue;
     Tensor p = l->params[i], g = p.grad();
-    if (!g.defined() || p.numel() == 0) continue;
     TORCH_CHECK(!g.is_sparse(), "adamw: sparse gradients are not supported");
     TORCH_CHECK(same_gpu(first, p) && same_gpu(first, g) && g.numel() == p.numel() && g.sizes() == p.sizes(), "adamw: a gradient does not match its parameter");
     const bool p16 = is_bf16(p, "adamw"), g16 = is_bf16(g, "adamw");
@@ -458,21 +459,15 @@ int64_t adamw_list_step(const std::shared_ptr<AdamwList>& l, double lr, const op
       back.emplace_back(p, c);
       p = c;
     }
-    const int64_t chunks = (p.numel() + adb200::kAdamwChunk - 1) / adb200::kAdamwChunk;
-    TORCH_CHECK(chunks < (1LL << 30), "adamw: a parameter is too large");
     Batch* b = nullptr;
     for (Batch& c : batches)
-      if (c.p16 == p16 && c.g16 == g16 && c.table->count < adb200::kAdamwMost && c.table->first[c.table->count] + chunks < (1LL << 30)) b = &c;
+      if (c.p16 == p16 && c.g16 == g16 && (int)c.tensors.size() < adb200::kAdamwMost) b = &c;
     if (b == nullptr) {
-      batches.push_back({p16, g16, std::make_unique<adb200::AdamwTable>()});
+      batches.push_back({p16, g16, {}});
       b = &batches.back();
-      b->table->count = 0;
-      b->table->first[0] = 0;
+      b->tensors.reserve(std::min<size_t>(l->params.size(), adb200::kAdamwMost));
     }
-    adb200::AdamwTable& t = *b->table;
-    t.t[t.count] = {p.data_ptr(), g.data_ptr(), p.numel(), l->places[i]};
-    t.first[t.count + 1] = t.first[t.count] + (int)chunks;
-    ++t.count;
+    b->tensors.push_back({p.data_ptr(), g.data_ptr(), p.numel(), l->places[i]});
   }
   const bool bits8 = l->m_scale.defined();
   const adb200::AdamwMoments mo{l->m.data_ptr(), l->r.data_ptr(), bits8 ? l->m_scale.data_ptr<float>() : nullptr, bits8 ? l->r_scale.data_ptr<float>() : nullptr};
@@ -480,7 +475,7 @@ int64_t adamw_list_step(const std::shared_ptr<AdamwList>& l, double lr, const op
                          reinterpret_cast<long long*>(l->step.data_ptr<int64_t>()), 0};
   for (size_t k = 0; k < batches.size(); ++k) {
     rule.advance = k + 1 == batches.size();
-    launched(adb200::adamw_list_step(*batches[k].table, batches[k].p16, batches[k].g16, mo, rule, st), "adamw");
+    launched(adb200::adamw_list_step(batches[k].tensors.data(), (int)batches[k].tensors.size(), batches[k].p16, batches[k].g16, mo, rule, st), "adamw");
   }
   for (auto& b : back) {
     at::NoGradGuard no_grad;
