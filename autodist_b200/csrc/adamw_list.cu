@@ -34,31 +34,33 @@ template <int MOST> struct Table {
 static_assert(sizeof(Table<kAdamwMost>) + 256 <= 32764, "kernel parameters");
 
 // 64 mixed bits of a counter, as the dropout decisions use them
-__device__ __forceinline__ uint64_t mixed(uint64_t seed, uint64_t i) {
-  uint64_t x = seed + i * 0x9E3779B97F4A7C15ull;
+constexpr uint64_t kGolden = 0x9E3779B97F4A7C15ull;
+__device__ __forceinline__ uint64_t mixed(uint64_t x) {
   x ^= x >> 30; x *= 0xBF58476D1CE4E5B9ull;
   x ^= x >> 27; x *= 0x94D049BB133111EBull;
   return x ^ (x >> 31);
 }
 
+// two last bits off at most, of a step that is itself small beside the parameter
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 
-// The e4m3 code of v (|v| <= 448, or a rounding more), rounded up where the cut-off part and u = (bits16 + 1/2) / 65536 add up to one. Codes are
-// a float's sign, exponent and upper three bits of the fraction: u is added below those, and what carries over is the rounding. Sizes
-// below 2^-6, whose codes are multiples of 2^-9, are moved up by 2^-6 first, where the steps are the same.
-__device__ __forceinline__ uint32_t round_random(float v, uint32_t bits16) {
-  const float size = fabsf(v);
-  const bool small = size < 0.015625f;
-  const uint32_t at = __float_as_uint(small ? __fadd_rz(size, 0.015625f) : size) + (bits16 << 4) + 8u;
-  uint32_t code = (at >> 20) - (small ? 968u : 960u);
-  code = min(code, 126u);                                // 448
-  if (code == 0u && size > 0.f) code = 1u;
-  if (size != size) code = 127u;
-  return code | (__float_as_uint(v) >> 24 & 0x80u);
+// The e4m3 code of a size (at most 448 and seven last bits), rounded up where the cut-off part and u = (bits16 + 1/2) / 65536 add up to one;
+// `random`: 16 bits << 4 | 8. A code is a float's exponent and upper three bits of the fraction. Times 2^-120 the two types' exponents
+// coincide, their subnormal numbers included (what is cut off there is below u's last bit), so that u is added below the fraction and
+// what carries over is the rounding: 448 has no lower bits that could carry past the largest code. Nothing but zero becomes zero.
+__device__ __forceinline__ uint32_t round_random(float size, uint32_t random) {
+  uint32_t code = (__float_as_uint(__fmul_rz(size, 7.52316384526264e-37f)) + random) >> 20;
+  if (size > 0.f) code = max(code, 1u);
+  return code;
 }
 
 // Two e4m3 codes of a word's lower half
@@ -79,7 +81,7 @@ __device__ Step step_of(const AdamwRule& r, long long t) {
   s.rate = (float)(lr / (1.0 - pow(r.b1, (double)t)));
   s.spread = (float)(1.0 / sqrt(1.0 - pow(r.b2, (double)t)));
   s.b1 = (float)r.b1; s.c1 = (float)(1.0 - r.b1); s.b2 = (float)r.b2; s.c2 = (float)(1.0 - r.b2); s.eps = (float)r.eps;
-  s.key = mixed(r.seed, (uint64_t)t);
+  s.key = mixed(r.seed + (uint64_t)t * kGolden);
   return s;
 }
 // Moments and parameter of one element; `root`: of the new second moment. The moments' roundings are spelled out, so that every kernel and
@@ -88,7 +90,7 @@ __device__ __forceinline__ void update(const Step& s, float& p, float g, float& 
   m = __fadd_rn(__fmul_rn(s.b1, m), __fmul_rn(s.c1, g));
   v = __fadd_rn(__fmul_rn(s.b2, v), __fmul_rn(s.c2, __fmul_rn(g, g)));
   root = __fsqrt_rn(v);
-  p = fmaf(p, s.decay, -s.rate * __fdividef(m, fmaf(root, s.spread, s.eps)));
+  p = fmaf(-s.rate * m, rcp_fast(fmaf(root, s.spread, s.eps)), p * s.decay);
 }
 
 // Eight neighbouring elements, of which `n` are there (8 or more: all, on 16 bytes).
@@ -137,7 +139,7 @@ __device__ __forceinline__ void store8(bf16* p, int n, bool whole, const float* 
 // A warp updates 256 elements at a time, a lane eight neighbours of them, so that the largest moments are found in registers and every byte
 // moves once. Blocks walk along the list's chunks: what a step's elements share (two powers in double) is computed once for each.
 template <typename P, typename G, bool BITS8, int MOST>
-__global__ void __launch_bounds__(kThreads) adamw_list_kernel(const __grid_constant__ Table<MOST> table, const AdamwMoments mo, const AdamwRule rule) {
+__global__ void __launch_bounds__(kThreads, 4) adamw_list_kernel(const __grid_constant__ Table<MOST> table, const AdamwMoments mo, const AdamwRule rule) {
   __shared__ Step shared;
   pdl_sync();
   if (threadIdx.x == 0) shared = step_of(rule, rule.step[0] + 1);
@@ -181,28 +183,39 @@ __global__ void __launch_bounds__(kThreads) adamw_list_kernel(const __grid_const
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         update(s, p[j], g[j], m[j], v[j], root[j]);
-        if (BITS8 && j < n) {
+        if (BITS8) {                                     // elements that are not there are zeros, as are their moments
           m_most = max_nan(m_most, fabsf(m[j]));
           r_most = max_nan(r_most, root[j]);
         }
       }
       store8(params + i, n, whole, p);
       if (BITS8) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          m_most = max_nan(m_most, __shfl_xor_sync(0xffffffffu, m_most, o));
-          r_most = max_nan(r_most, __shfl_xor_sync(0xffffffffu, r_most, o));
-        }
+        // sizes compare as their bits do, NaN above infinity
+        m_most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m_most)));
+        r_most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(r_most)));
         const bool m_held = !(m_most < kTiniest), r_held = !(r_most < kTiniest);
         const float m_inv = m_held ? __fmul_rn(__frcp_rn(m_most), kE4m3Max) : 0.f, r_inv = r_held ? __fmul_rn(__frcp_rn(r_most), kE4m3Max) : 0.f;
         uint32_t mc[2] = {0u, 0u}, rc[2] = {0u, 0u};
+        uint64_t counter = s.key + ((uint64_t)q >> 1) * kGolden;               // a hash for two neighbours
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint64_t word = mixed(s.key, (uint64_t)(q + j) >> 1);          // shared by two neighbours
-          const uint32_t bits = (uint32_t)(word >> (32 * (j & 1)));
-          const bool there = j < n;
-          mc[j >> 2] |= (there ? round_random(__fmul_rn(m[j], m_inv), bits & 0xFFFFu) : 0u) << (8 * (j & 3));
-          rc[j >> 2] |= (there ? round_random(__fmul_rn(root[j], r_inv), bits >> 16) : 0u) << (8 * (j & 3));
+        for (int j = 0; j < 8; j += 2, counter += kGolden) {
+          const uint64_t word = mixed(counter);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t bits = (uint32_t)(word >> (32 * h)), at = 8 * ((j + h) & 3);
+            const float x = __fmul_rn(m[j + h], m_inv);
+            const uint32_t code = round_random(fabsf(x), (bits << 4 & 0xFFFF0u) | 8u) | (__float_as_uint(x) >> 24 & 0x80u);
+            mc[j >> 2] += code << at;
+            rc[j >> 2] += round_random(__fmul_rn(root[j + h], r_inv), (bits >> 12 & 0xFFFF0u) | 8u) << at;
+          }
+        }
+        // a block with a moment that is not finite is spoilt as a whole where its scale is NaN, else where the moment is not finite
+        if (!(m_most < __int_as_float(0x7F800000)) || !(r_most < __int_as_float(0x7F800000))) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (isnan(m[j] * m_inv)) mc[j >> 2] |= 0x7Fu << (8 * (j & 3));
+            if (isnan(root[j] * r_inv)) rc[j >> 2] |= 0x7Fu << (8 * (j & 3));
+          }
         }
         *reinterpret_cast<uint2*>(static_cast<uint8_t*>(mo.m) + q) = make_uint2(mc[0], mc[1]);
         *reinterpret_cast<uint2*>(static_cast<uint8_t*>(mo.r) + q) = make_uint2(rc[0], rc[1]);
