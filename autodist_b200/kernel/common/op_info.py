@@ -12,6 +12,7 @@ SLOT_NAMES = {
     "SGD": ("momentum_buffer",),
     "Adam": ("exp_avg", "exp_avg_sq", "max_exp_avg_sq"),
     "AdamW": ("exp_avg", "exp_avg_sq", "max_exp_avg_sq"),
+    "ListAdamW": ("exp_avg", "exp_avg_sq"),       # in fp32, through the optimizer's slots_of / load_slots
     "Adagrad": ("sum",),
     "RMSprop": ("square_avg", "momentum_buffer", "grad_avg"),
     "Adadelta": ("square_avg", "acc_delta"),

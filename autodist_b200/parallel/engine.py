@@ -559,7 +559,8 @@ class StepEngine:
             full: Dict[str, torch.Tensor] = {}
             if local is not None:
                 for t in self._targets:
-                    st = local.state.get(t.param)
+                    # an optimizer with a state layout of its own says what its slots are
+                    st = local.slots_of(t.param) if hasattr(local, "slots_of") else local.state.get(t.param)
                     if not st:
                         continue
                     for slot in names:
@@ -606,10 +607,13 @@ class StepEngine:
                         loaded[slot] = (src if t.part is None else t.part.view(src)).clone()
                 if not loaded:
                     continue
-                st = local.state[t.param]
-                st.update(loaded)
                 # The writer only knows the step counters of the parts it owned; the rest took as many steps.
                 step = slots.get(f"{t.var_name[:-2]}/step", default_step)
+                if hasattr(local, "load_slots"):
+                    local.load_slots(t.param, loaded, float(step))
+                    continue
+                st = local.state[t.param]
+                st.update(loaded)
                 st["step"] = torch.as_tensor(float(step))
 
     def close(self):
