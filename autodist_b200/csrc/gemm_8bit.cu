@@ -14,6 +14,7 @@
 #include <cuda.h>
 #include <cuda_bf16.h>
 
+#include <array>
 #include <mutex>
 
 #include "gemm_epilogue.cuh"
@@ -67,6 +68,12 @@ __device__ __forceinline__ void give_up(volatile int* abort_flag, int* error, in
 __device__ __forceinline__ float4 four_of(const float* v, int i, int n) {
   if (i + 4 <= n) return __ldg(reinterpret_cast<const float4*>(v + i));
   return make_float4(i < n ? v[i] : 0.f, i + 1 < n ? v[i + 1] : 0.f, i + 2 < n ? v[i + 2] : 0.f, 0.f);
+}
+
+// Two of them from an even place on.
+__device__ __forceinline__ float2 two_of(const float* v, int i, int n) {
+  if (i + 2 <= n) return __ldg(reinterpret_cast<const float2*>(v + i));
+  return make_float2(i < n ? v[i] : 0.f, 0.f);
 }
 
 // ------------------------------------------------------------------------------------------------ tiles
@@ -338,15 +345,26 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
     int as = 0; uint32_t aphase = 0; bool ok = true;
     for (long long t = pair; t < total && ok; t += pairs) {
       const int row0 = (int)(t % tiles_m) * 256 + (int)rank * 128 + q * 32, col0 = (int)(t / tiles_m) * P_BN + part * 128;
-      const float sx = row0 + lane < a.M ? __ldg(a.scales + row0 + lane) : 0.f;
+      // what belongs to the tile's rows and columns comes while the tile is still being multiplied: in the fragment layout a lane has columns
+      // 8 k + 2 (lane % 4) and the one beside of the rows lane / 4 + 8 i
+      float sx[4];
+      float2 sw[16], bias[16];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sx[i] = row0 + lane / 4 + 8 * i < a.M ? __ldg(a.scales + row0 + lane / 4 + 8 * i) : 0.f;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const int col = col0 + 8 * k + 2 * (lane & 3);
+        sw[k] = two_of(a.weight_scales, col, a.N);
+        bias[k] = a.bias != nullptr ? two_of(a.bias, col, a.N) : make_float2(0.f, 0.f);
+      }
       if (!mbar_wait(&tfull[as], aphase, abort_flag)) { ok = false; break; }
       tc_fence_after();
       const uint32_t t_w = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(as * P_BN + part * 128);
-#pragma unroll 1
+#pragma unroll
       for (int c = 0; c < 4; ++c) {                        // 32 columns; two of them fill a box
-        float v[32];
+        uint32_t v[32];
         __syncwarp();
-        tmem_ld32(t_w + c * 32, v);
+        tmem_ld_frag32(t_w + c * 32, v);
         if (c == 3) {                                      // this warp has read its part of the accumulator
           tc_fence_before();
           if (elect_one()) mbar_arrive_cluster(map_to_cta(smem_u32(&tempty[as]), 0));
@@ -358,18 +376,15 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constan
         }
         const uint32_t buf = box + (uint32_t)(c >> 1) * 4096u;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t w[4];
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t r = (uint32_t)lane / 4 + 8 * i;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int i = 8 * j + 4 * h;
-            const float4 sw = four_of(a.weight_scales, col + i, a.N);
-            const float4 bias = a.bias != nullptr ? four_of(a.bias, col + i, a.N) : make_float4(0.f, 0.f, 0.f, 0.f);
-            w[2 * h] = pack2(fmaf(v[i], sx * sw.x, bias.x), fmaf(v[i + 1], sx * sw.y, bias.y));
-            w[2 * h + 1] = pack2(fmaf(v[i + 2], sx * sw.z, bias.z), fmaf(v[i + 3], sx * sw.w, bias.w));
+          for (int k = 0; k < 4; ++k) {
+            const float2 w = sw[c * 4 + k], b = bias[c * 4 + k];
+            const float x = __uint_as_float(v[(i / 2) * 16 + k * 4 + (i % 2) * 2]), y = __uint_as_float(v[(i / 2) * 16 + k * 4 + (i % 2) * 2 + 1]);
+            const uint32_t chunk = (uint32_t)((c & 1) * 4 + k);
+            sts1(buf + r * 128u + ((chunk ^ (r & 7)) << 4) + ((uint32_t)lane & 3u) * 4u, pack2(fmaf(x, sx[i] * w.x, b.x), fmaf(y, sx[i] * w.y, b.y)));
           }
-          const uint32_t chunk = (uint32_t)((c & 1) * 4 + j);
-          st_shared_v4(buf + (uint32_t)lane * 128u + ((chunk ^ (uint32_t)(lane & 7)) << 4), w[0], w[1], w[2], w[3]);
         }
         if (c & 1) {
           const int first = col - 32;
@@ -489,22 +504,61 @@ cudaError_t launch_pairs(const Gemm8Args& a, cudaStream_t st) {
   return cudaLaunchKernelEx(&cfg, gemm8_pair_kernel, tm_x, tm_w, tm_y, a, boxes);
 }
 
+// Clusters of `split` tiles' CTAs that are resident at once: one CTA fills an SM at every width.
+int clusters_of(int split) {
+  static const std::array<int, 9> counts = [] {
+    std::array<int, 9> c{};
+    c[1] = sm_count();
+    if (cudaFuncSetAttribute(gemm8_tile_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, TileCfg<128>::SMEM) != cudaSuccess) return c;
+    for (int s = 2; s <= 8; ++s) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3((unsigned)(sm_count() / s * s));
+      cfg.blockDim = dim3(kTileThreads);
+      cfg.dynamicSmemBytes = TileCfg<128>::SMEM;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = (unsigned)s; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr; cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&c[s], gemm8_tile_kernel<128>, &cfg) != cudaSuccess) { (void)cudaGetLastError(); c[s] = 0; }
+    }
+    return c;
+  }();
+  return counts[split];
+}
+
+// Which kernel, tile and split: the shortest estimate in us. A wave of tiles costs its K blocks, more of them the more SMs take part (their
+// copies share the L2), and every wave but the last the draining of its tiles; a split adds the exchange. The constants are fitted to
+// 3157 launches of 256 products of 1 to 4096 rows, 256 to 4096 codes and 256 to 8192 outputs (replayed back to back); the chosen
+// launches take 1.4 % more time in sum than the fastest of each product:
+//   8 x 1024 x 8192 4.1 with 16 columns, 5.3 with 128; 8 x 4096 x 1000 4.4 split eight ways, 7.3 whole; 128 x 1024 x 8192 5.5 with 64 columns,
+//   7.2 with 128, 7.5 on pairs; 1024 x 1024 x 8192 27.6 with 128 columns, 11.5 on pairs
+void choose(const Gemm8Args& a, int* bn, int* split) {
+  struct Cost { int bn; double base, block, load, wave, exchange; };
+  static const Cost costs[5] = {{16, 2.85, 0.14, 0.03, 2.46, 0.96}, {32, 3.15, 0.13, 0.06, 2.85, 0.87}, {64, 3.49, 0.13, 0.12, 3.27, 0.80},
+                                {128, 3.89, 0.13, 0.27, 3.73, 0.74}, {512, 5.02, 0.27, 0.09, 1.27, 0.0}};
+  const long long num_kb = (a.K + KB - 1) / KB;
+  double best = 1e30;
+  for (const Cost& c : costs) {
+    const bool pairs = c.bn == 512;
+    const long long tiles = pairs ? (long long)((a.M + 255) / 256) * ((a.N + 255) / 256) : (long long)((a.M + c.bn - 1) / c.bn) * ((a.N + 127) / 128);
+    for (int s = 1; s <= (pairs ? 1 : 8) && s <= num_kb; ++s) {
+      const long long slots = pairs ? sm_count() / 2 : clusters_of(s);
+      if (slots <= 0 || (s > 1 && tiles > slots)) continue;          // splitting more than what is resident at once only adds exchanges
+      const double waves = (double)((tiles + slots - 1) / slots), blocks = waves * (double)((num_kb + s - 1) / s), load = tiles < slots ? (double)tiles / slots : 1.0;
+      const double us = c.base + blocks * (c.block + c.load * load) + c.wave * (waves - 1) + (s > 1 ? c.exchange : 0.0);
+      if (us < best) { best = us; *bn = c.bn; *split = s; }
+    }
+  }
+}
+
 }  // namespace
 
 cudaError_t gemm_8bit(const Gemm8Args& a, int bn, int split, cudaStream_t st) {
   if (a.M <= 0 || a.N <= 0) return cudaSuccess;
   const int num_kb = (a.K + KB - 1) / KB;
-  if (bn == 0) {
-    const long long pair_tiles = (long long)((a.M + 255) / 256) * ((a.N + 255) / 256);
-    if (a.M > 256 && pair_tiles >= 48) bn = 512;
-    else bn = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
-  }
+  if (bn == 0) choose(a, &bn, &split);
   if (bn == 512) return launch_pairs(a, st);
-  const long long tiles = (long long)((a.M + bn - 1) / bn) * ((a.N + 127) / 128);
-  if (split == 0) {
-    split = 1;
-    while (split < 8 && tiles * (split + 1) <= sm_count() && num_kb >= 2 * (split + 1)) ++split;
-  }
+  if (split == 0) split = 1;
   if (split < 1 || split > 8 || split > num_kb) return cudaErrorInvalidValue;
   switch (bn) {
     case 16: return launch_tiles<16>(a, split, st);

@@ -243,7 +243,7 @@ Tensor gemm_8bit(const Tensor& codes, const Tensor& scales, const Tensor& weight
   const Tensor x = aligned_codes(codes, "the rows"), w = aligned_codes(weight_codes, "the weight");
   const int64_t M = x.size(0), N = w.size(0);
   TORCH_CHECK(M < (1LL << 31) && N < (1LL << 31), "linear_8bit: too many rows");
-  TORCH_CHECK(scales.scalar_type() == at::kFloat && scales.numel() == M && weight_scales.scalar_type() == at::kFloat && weight_scales.numel() == N,
+  TORCH_CHECK(scales.scalar_type() == at::kFloat && scales.sizes() == codes.sizes().slice(0, codes.dim() - 1) && weight_scales.dim() == 1 && weight_scales.scalar_type() == at::kFloat && weight_scales.numel() == N,
               "linear_8bit: an fp32 scale for each row needed");
   TORCH_CHECK(!bias.has_value() || (bias->scalar_type() == at::kFloat && bias->numel() == N), "linear_8bit: an fp32 bias for each output needed");
   TORCH_CHECK(error.scalar_type() == at::kInt && error.numel() >= 1, "linear_8bit: an int32 word needed");

@@ -65,11 +65,15 @@ def _norm_again(s, weight, eps, dy, ds):
 def rms_norm(x, weight, residual=None, eps=1e-6):
     """``s * rsqrt(mean(s^2) + eps) * weight`` over the last dimension, with ``s = x``, or ``s = x + residual`` rounded to their type; then
     ``(norm, s)`` is returned. bf16 or fp32; the weight in fp32 or in the input's type. Sums are fp32."""
-    _check_norm("rms_norm", x, weight, residual)
     if not _kernels(x):
+        _check_norm("rms_norm", x, weight, residual)
         y, s = _norm_plain(x, weight, residual, eps)
         return y.to(x.dtype) if residual is None else (y.to(x.dtype), s)
-    y, s = ops.ext(required=True).rms_norm(x, weight, residual, eps)
+    try:
+        y, s = ops.ext(required=True).rms_norm(x, weight, residual, eps)
+    except RuntimeError:                        # the binding checks all of this too; here the argument at fault is named
+        _check_norm("rms_norm", x, weight, residual)
+        raise
     return y if residual is None else (y, s)
 
 
@@ -88,12 +92,16 @@ def rms_norm_8bit(x, weight, residual=None, eps=1e-6):
     """``rms_norm`` with its output in 8 bits: ``(codes, scales)``, or ``(codes, scales, s)`` with a residual. ``codes`` (``float8_e4m3fn``)
     times its row's fp32 scale is the norm's output, the row's largest element being 448 scales; rows of zeros have the scale 0. Rows of
     ``codes`` start on 16-byte boundaries, as ``linear_8bit`` reads them. Not differentiable."""
-    _check_norm("rms_norm_8bit", x, weight, residual)
     _no_gradient("rms_norm_8bit", x, weight, residual)
     if not _kernels(x):
+        _check_norm("rms_norm_8bit", x, weight, residual)
         y, s = _norm_plain(x, weight, residual, eps)
         return _codes_plain(y) if residual is None else _codes_plain(y) + (s,)
-    codes, scales, s = ops.ext(required=True).rms_norm_8bit(x, weight, residual, eps)
+    try:
+        codes, scales, s = ops.ext(required=True).rms_norm_8bit(x, weight, residual, eps)
+    except RuntimeError:
+        _check_norm("rms_norm_8bit", x, weight, residual)
+        raise
     return (codes, scales) if residual is None else (codes, scales, s)
 
 
@@ -109,9 +117,7 @@ def quantize_rows(x):
 
 
 # ---------------------------------------------------------------------------------------------------------------- product in 8 bits
-def linear_8bit(codes, scales, weight_codes, weight_scales, bias=None):
-    """``(codes * scales) @ (weight_codes * weight_scales).T + bias`` in bf16 for rows ``[..., K]`` and a weight ``[N, K]`` of
-    ``float8_e4m3fn`` with an fp32 scale each (``rms_norm_8bit``, ``quantize_rows``). Products are exact, sums fp32. Not differentiable."""
+def _check_linear(codes, scales, weight_codes, weight_scales, bias):
     if codes.dtype != torch.float8_e4m3fn or weight_codes.dtype != torch.float8_e4m3fn:
         raise TypeError(f"linear_8bit: float8_e4m3fn rows and weight needed, got {codes.dtype} and {weight_codes.dtype}")
     if codes.dim() < 1 or weight_codes.dim() != 2 or codes.shape[-1] != weight_codes.shape[1] or codes.shape[-1] < 1:
@@ -121,10 +127,20 @@ def linear_8bit(codes, scales, weight_codes, weight_scales, bias=None):
         raise ValueError("linear_8bit: an fp32 scale for each row of both sides needed")
     if bias is not None and (bias.dtype != torch.float32 or bias.shape != weight_scales.shape):
         raise ValueError("linear_8bit: an fp32 bias for each output needed")
+
+
+def linear_8bit(codes, scales, weight_codes, weight_scales, bias=None):
+    """``(codes * scales) @ (weight_codes * weight_scales).T + bias`` in bf16 for rows ``[..., K]`` and a weight ``[N, K]`` of
+    ``float8_e4m3fn`` with an fp32 scale each (``rms_norm_8bit``, ``quantize_rows``). Products are exact, sums fp32. Not differentiable."""
     _no_gradient("linear_8bit", scales, weight_scales, bias)
     if codes.is_cuda:
         from autodist_b200.ops.functional import _error_flag
-        return ops.ext(required=True).gemm_8bit(codes, scales, weight_codes, weight_scales, bias, _error_flag(codes.device))
+        try:
+            return ops.ext(required=True).gemm_8bit(codes, scales, weight_codes, weight_scales, bias, _error_flag(codes.device))
+        except RuntimeError:
+            _check_linear(codes, scales, weight_codes, weight_scales, bias)
+            raise
+    _check_linear(codes, scales, weight_codes, weight_scales, bias)
     y = F.linear(codes.float(), weight_codes.float()) * scales[..., None] * weight_scales
     return (y if bias is None else y + bias).to(torch.bfloat16)
 
@@ -151,13 +167,7 @@ def _scan_again(x, forget, input_gate, state, reset, forget_bias, dy, dlast):
     return _differentiated_again(lambda *a: _scan_plain(*a, reset, forget_bias), (x, forget, input_gate, state), (dy, dlast))
 
 
-def gated_recurrence(x, forget, input_gate=None, state=None, reset=None, forget_bias=0.0):
-    """``h_t = f_t * h_{t-1} + u_t * x_t`` channel by channel over ``[batch, steps, channels]``: ``(h in x's type, last state in fp32)``.
-
-    ``f = sigmoid(forget + forget_bias)``; ``u = sigmoid(input_gate)``, or ``1 - f`` without one. ``state``: fp32 ``[batch, channels]``, the
-    state in front of the first step (zeros without one); pass the last state on to continue, one token at a time if need be.
-    ``reset``: bool ``[batch, steps]``, the steps that forget the state in front of them (a document begins). bf16 or fp32; strided views,
-    such as slices of one projection, are read in place. States are fp32 throughout; the backward pass computes them again."""
+def _check_scan(x, forget, input_gate, state, reset):
     if x.dtype not in _STREAM_TYPES:
         raise TypeError(f"gated_recurrence: bf16 or fp32 needed, got {x.dtype}")
     if x.dim() != 3:
@@ -169,9 +179,23 @@ def gated_recurrence(x, forget, input_gate=None, state=None, reset=None, forget_
         raise ValueError(f"gated_recurrence: an fp32 state [batch, channels] needed, got {tuple(state.shape)} {state.dtype}")
     if reset is not None and (reset.dtype != torch.bool or reset.shape != x.shape[:2]):
         raise ValueError(f"gated_recurrence: a bool reset [batch, steps] needed, got {tuple(reset.shape)} {reset.dtype}")
+
+
+def gated_recurrence(x, forget, input_gate=None, state=None, reset=None, forget_bias=0.0):
+    """``h_t = f_t * h_{t-1} + u_t * x_t`` channel by channel over ``[batch, steps, channels]``: ``(h in x's type, last state in fp32)``.
+
+    ``f = sigmoid(forget + forget_bias)``; ``u = sigmoid(input_gate)``, or ``1 - f`` without one. ``state``: fp32 ``[batch, channels]``, the
+    state in front of the first step (zeros without one); pass the last state on to continue, one token at a time if need be.
+    ``reset``: bool ``[batch, steps]``, the steps that forget the state in front of them (a document begins). bf16 or fp32; strided views,
+    such as slices of one projection, are read in place. States are fp32 throughout; the backward pass computes them again."""
     if not math.isfinite(forget_bias):
         raise ValueError(f"gated_recurrence: a finite forget_bias needed, got {forget_bias}")
     if not _kernels(x):
+        _check_scan(x, forget, input_gate, state, reset)
         return _scan_plain(x, forget, input_gate, state, reset, forget_bias)
-    y, last, _ = ops.ext(required=True).gated_scan(x, forget, input_gate, state, reset, forget_bias)
+    try:
+        y, last, _ = ops.ext(required=True).gated_scan(x, forget, input_gate, state, reset, forget_bias)
+    except RuntimeError:
+        _check_scan(x, forget, input_gate, state, reset)
+        raise
     return y, last
