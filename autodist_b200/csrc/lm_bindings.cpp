@@ -437,6 +437,26 @@ std::shared_ptr<AdamwList> adamw_list(std::vector<Tensor> params, std::vector<in
   return list;
 }
 
+// Each parameter's moments (and their scales) as views of the flat ones, the moments in the parameter's shape.
+std::vector<std::vector<Tensor>> adamw_views(const std::shared_ptr<AdamwList>& l) {
+  std::vector<std::vector<Tensor>> views;
+  views.reserve(l->params.size());
+  for (size_t i = 0; i < l->params.size(); ++i) {
+    const Tensor& p = l->params[i];
+    std::vector<int64_t> strides(p.dim());
+    int64_t n = 1;
+    for (int64_t d = p.dim() - 1; d >= 0; --d) { strides[d] = n; n *= p.size(d); }
+    const int64_t block = l->places[i] / adb200::kAdamwBlock, blocks = (n + adb200::kAdamwBlock - 1) / adb200::kAdamwBlock;
+    std::vector<Tensor> v{l->m.as_strided(p.sizes(), strides, l->places[i]), l->r.as_strided(p.sizes(), strides, l->places[i])};
+    if (l->m_scale.defined()) {
+      v.push_back(l->m_scale.narrow(0, block, blocks));
+      v.push_back(l->r_scale.narrow(0, block, blocks));
+    }
+    views.push_back(std::move(v));
+  }
+  return views;
+}
+
 // One step over the parameters that have a gradient. Returns how many kernels it launched.
 int64_t adamw_list_step(const std::shared_ptr<AdamwList>& l, double lr, const optional<Tensor>& lr_at, double b1, double b2, double eps, double wd) {
   const Tensor& first = l->params[0];
@@ -448,16 +468,21 @@ int64_t adamw_list_step(const std::shared_ptr<AdamwList>& l, double lr, const op
   std::vector<Tensor> held;                                  // gradients and parameters that had to be laid out
   std::vector<std::pair<Tensor, Tensor>> back;               // parameters to copy into, from their laid-out copies
   for (size_t i = 0; i < l->params.size(); ++i) {
-    if (!l->params[i].grad().defined() || l->params[i].numel() == 0) continue;
-    Tensor p = l->params[i], g = p.grad();
+    const Tensor &p = l->params[i], &g = p.grad();
+    const int64_t n = p.numel();
+    if (!g.defined() || n == 0) continue;
     TORCH_CHECK(!g.is_sparse(), "adamw: sparse gradients are not supported");
-    TORCH_CHECK(same_gpu(first, p) && same_gpu(first, g) && g.numel() == p.numel() && g.sizes() == p.sizes(), "adamw: a gradient does not match its parameter");
+    TORCH_CHECK(same_gpu(first, p) && same_gpu(first, g) && g.sizes() == p.sizes(), "adamw: a gradient does not match its parameter");
     const bool p16 = is_bf16(p, "adamw"), g16 = is_bf16(g, "adamw");
-    if (!g.is_contiguous()) held.push_back(g = g.contiguous());
+    const void* gp = g.data_ptr();
+    void* pp = p.data_ptr();
+    if (!g.is_contiguous()) {
+      held.push_back(g.contiguous());
+      gp = held.back().data_ptr();
+    }
     if (!p.is_contiguous()) {
-      Tensor c = p.detach().contiguous();
-      back.emplace_back(p, c);
-      p = c;
+      back.emplace_back(p, p.detach().contiguous());
+      pp = back.back().second.data_ptr();
     }
     Batch* b = nullptr;
     for (Batch& c : batches)
@@ -467,7 +492,7 @@ int64_t adamw_list_step(const std::shared_ptr<AdamwList>& l, double lr, const op
       b = &batches.back();
       b->tensors.reserve(std::min<size_t>(l->params.size(), adb200::kAdamwMost));
     }
-    b->tensors.push_back({p.data_ptr(), g.data_ptr(), p.numel(), l->places[i]});
+    b->tensors.push_back({pp, gp, n, l->places[i]});
   }
   const bool bits8 = l->m_scale.defined();
   const adb200::AdamwMoments mo{l->m.data_ptr(), l->r.data_ptr(), bits8 ? l->m_scale.data_ptr<float>() : nullptr, bits8 ? l->r_scale.data_ptr<float>() : nullptr};
@@ -500,6 +525,7 @@ void register_lm(pybind11::module& m) {
   m.def("gated_scan_bwd", &gated_scan_bwd);
   pybind11::class_<AdamwList, std::shared_ptr<AdamwList>>(m, "_AdamwList");
   m.def("adamw_list", &adamw_list);
+  m.def("adamw_views", &adamw_views);
   m.def("adamw_list_step", &adamw_list_step);
   m.attr("ADAMW_BLOCK") = adb200::kAdamwBlock;
 }

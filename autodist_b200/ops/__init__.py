@@ -52,7 +52,7 @@ def _copy_list_launches(taken, dst, src):
 class _Counting:
     """Thin proxy over the extension module that counts kernel-launching calls."""
     _NO_LAUNCH = {"ln_bwd_part_floats", "sampled_grad_chunks", "sampled_bias_chunks", "bce_logits_parts", "colsum_parts", "gemm_choice", "gemm_set_trace", "conv_set_trace", "MAX_COMM_BLOCKS",
-                  "adamw_list", "backward_kernels"}
+                  "adamw_list", "adamw_views", "backward_kernels"}
     #: kernels per call where that is not one: a number, or a function of the call's arguments
     _MULTI = {"ln_bwd": 2, "keyed_colsum": 2, "relu_bwd_colsum": 2, "bn_sums": 2, "bn_bwd": 2,
               "bn_fwd": lambda *a: 1 if a[9] is not None else 3, "bn_fwd_nchw": lambda *a: 1 if a[6] is not None else 3,       # sums given or not

@@ -109,10 +109,13 @@ class ListAdamW(torch.optim.Optimizer):
         if dev.type == "cuda" and total:
             own["list"] = ops.ext(required=True).adamw_list(own["params"], places, buffers["exp_avg"], buffers["exp_avg_sq"], buffers.get("exp_avg_scale"),
                                                             buffers.get("exp_avg_sq_scale"), own["step"], self.seed + index)
-        for p, o in zip(params, places):
-            n = p.numel()
-            self.state[p] = {k: b[o:o + n].view(p.shape) if b.numel() == total else b[o // BLOCK:(o + n + BLOCK - 1) // BLOCK] for k, b in buffers.items()}
-            self.state[p]["step"] = own["step"][:1]
+            views = ops.ext(required=True).adamw_views(own["list"])
+        else:
+            views = [[b[o:o + p.numel()].view(p.shape) if b.numel() == total else b[o // BLOCK:(o + _round_up(p.numel(), BLOCK)) // BLOCK] for b in buffers.values()]
+                     for p, o in zip(params, places)]
+        taken = own["step"][:1]
+        for p, v in zip(params, views):
+            self.state[p] = dict(zip(buffers, v), step=taken)
         return own
 
     @property
