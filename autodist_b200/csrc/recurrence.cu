@@ -17,6 +17,13 @@
 //                   whose warps hear from nobody (the inputs are read twice, but by as many blocks as the GPU holds); a chunk's block
 //                   folds those in front of its own. The order of joining is fixed.
 //
+// Measured (B200, replayed back to back, bf16; share of the copy rate by the bytes that have to move): 32 x 2048 x 1024 forward 72 us (0.85),
+// backward 136 (0.75); 1 x 65536 x 1024 127 (0.48; its inputs are read twice) and 182 (0.56); 128 x 20 x 2048 with an input gate 12.8
+// (0.50) and 18.7 (0.60); in fp32 1 x 32768 x 1024 106 and 152. What bounds them is issuing instructions, 19 a value forward and 39
+// backward, of which the memory would allow 33 and 55 with every issue slot taken: so values go in pairs, gates stay in registers
+// (8 or 16 steps of a warp: what 128 registers hold at 16 warps an SM), and inputs are read again from shared memory instead of
+// being kept (32 x 2048 x 1024 backward 156 -> 132).
+//
 // The states are not stored: the forward pass keeps them in fp32 in front of every tile of the backward pass, which walks the other way with
 // the same joining of dh and computes those in between again. States, gates and sums are fp32.
 #include "recurrence.h"
@@ -108,23 +115,26 @@ constexpr float kLog2e = 1.4426950408889634f;
 // finite: a gate shut by minus infinity still lets some 2^-126 through.
 //   bf16  the exponent in one rounding: e is off by |g| 2^-24 or so, far below what the rounding of g to 8 bits did to it
 //   fp32  what the product with log2(e) cut off is put back, so that e is off by the exponential's own two last bits
-template <int VEC> __device__ __forceinline__ F<VEC> reciprocal(F<VEC> d) {
-  // a step of Newton's: products of a thousand gates close to one show a bias of the approximation's last bit (1 x 65536 x 1024: the
-  // state's gradient 1.0e-6 off, 0.6e-6 with it)
-  const F<VEC> r = each(d, rcp_fast);
-  return fma(r, fma(mul(d, all<VEC>(-1.f)), r, all<VEC>(1.f)), r);
+// 1 / (1 + e). NEWTON, for the forget gates: a step of Newton's, without which products of a thousand gates close to one show a bias of the
+// approximation's last bit (1 x 65536 x 1024: the state's gradient 1.0e-6 off, 0.6e-6 with it). In single values: in pairs it cost
+// the backward pass 18 % of its time in registers moved about (32 x 2048 x 1024 132 -> 156 us, in single values 136).
+template <bool NEWTON, int VEC> __device__ __forceinline__ F<VEC> reciprocal(F<VEC> e) {
+  return each(add(e, all<VEC>(1.f)), [](float d) {
+    const float r = rcp_fast(d);
+    return NEWTON ? fmaf(r, fmaf(-d, r, 1.f), r) : r;
+  });
 }
-template <typename T, int VEC> struct Gate;
-template <int VEC> struct Gate<bf16, VEC> {
+template <typename T, int VEC, bool NEWTON> struct Gate;
+template <int VEC, bool NEWTON> struct Gate<bf16, VEC, NEWTON> {
   F<VEC> bias;
   __device__ __forceinline__ explicit Gate(float b) : bias(all<VEC>(-kLog2e * b)) {}
   __device__ __forceinline__ void operator()(F<VEC> g, F<VEC>& f, F<VEC>& n) const {
     const F<VEC> e = each(fma(g, all<VEC>(-kLog2e), bias), [](float x) { return exp2_fast(min_nan(x, 126.f)); });
-    f = reciprocal(add(e, all<VEC>(1.f)));
+    f = reciprocal<NEWTON>(e);
     n = mul(e, f);
   }
 };
-template <int VEC> struct Gate<float, VEC> {
+template <int VEC, bool NEWTON> struct Gate<float, VEC, NEWTON> {
   F<VEC> bias;
   __device__ __forceinline__ explicit Gate(float b) : bias(all<VEC>(b)) {}
   __device__ __forceinline__ void operator()(F<VEC> g, F<VEC>& f, F<VEC>& n) const {
@@ -133,7 +143,7 @@ template <int VEC> struct Gate<float, VEC> {
     const F<VEC> cut = fma(z, all<VEC>(-1.925963033500e-08f), fma(z, all<VEC>(-kLog2e), mul(x, all<VEC>(-1.f))));     // log2(e) is kLog2e + 1.926e-8
     const F<VEC> p = each(x, exp2_fast);
     const F<VEC> e = fma(p, mul(cut, all<VEC>(0.69314718f)), p);
-    f = reciprocal(add(e, all<VEC>(1.f)));
+    f = reciprocal<NEWTON>(e);
     n = mul(e, f);
   }
 };
@@ -248,6 +258,38 @@ __device__ __forceinline__ uint32_t load_cuts(const ScanArgs& a, int b, int t0, 
   return __ballot_sync(0xffffffffu, cut);
 }
 
+// A few steps, a single token among them: a thread walks through its channels' by itself.
+constexpr int kFew = 4;
+template <typename T, int VEC, bool GATE>
+__global__ void __launch_bounds__(256) scan_few_kernel(const ScanArgs a, T* __restrict__ y, float* __restrict__ last, float* __restrict__ kept) {
+  typedef Lane<T, VEC> L;
+  typedef F<VEC> V;
+  pdl_sync();
+  const int across = a.channels / VEC;
+  const long long at = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  if (at >= (long long)across * a.batch) return;
+  const int b = (int)(at / across), c = (int)(at % across) * VEC;
+  const long long state_at = (long long)b * a.channels + c;
+  V h = a.state != nullptr ? load_f(a.state + state_at, static_cast<V*>(nullptr)) : all<VEC>(0.f);
+  if (kept != nullptr && a.steps > 0) store_f(kept + state_at, h);            // all steps lie in one tile
+  const Gate<T, VEC, true> forget(a.forget_bias);
+  const Gate<T, VEC, false> input(0.f);
+  auto read = [&](const ScanView& v, int t) { return L::unpack(*reinterpret_cast<const typename L::Raw*>(static_cast<const T*>(v.p) + b * v.batch + t * v.step + c)); };
+  for (int t = 0; t < a.steps; ++t) {
+    V f, n;
+    forget(read(a.forget, t), f, n);
+    if constexpr (GATE) {
+      V m;
+      input(read(a.input, t), n, m);
+    }
+    const V w = mul(n, read(a.x, t));
+    const bool cut = a.reset != nullptr && a.reset[b * a.reset_batch + t * a.reset_step] != 0;
+    h = cut ? w : fma(f, h, w);
+    L::store(y + ((long long)b * a.steps + t) * a.channels + c, h);
+  }
+  store_f(last + state_at, h);
+}
+
 // Chunks of `tiles` tiles each that a sequence is cut into. runs: what the `pieces` of each do to a state (forward) or to dh (backward),
 // [count * pieces][2][batch][channels].
 struct Chunks {
@@ -293,7 +335,8 @@ scan_chunks_kernel(const ScanArgs a, const ScanView dy, const int wide, const in
   };
 #pragma unroll
   for (int k = 0; k < R::SLOTS - 1; ++k) request(k);
-  const Gate<T, VEC> forget(a.forget_bias), input(0.f);
+  const Gate<T, VEC, true> forget(a.forget_bias);
+  const Gate<T, VEC, false> input(0.f);
   uint32_t cuts = 0, next_cuts = 0;
   if (CUT) next_cuts = load_cuts<STEPS>(a, at.b, t_first, at.lane);
   Run<VEC> sum = {all<VEC>(1.f), all<VEC>(0.f)};
@@ -382,7 +425,8 @@ scan_fwd_kernel(const ScanArgs a, T* __restrict__ y, float* __restrict__ last, f
   if (at.live)
 #pragma unroll 4
     for (int z = 0; z < at.chunk * ch.pieces; ++z) carry = after<CUT>(ch.run<VEC>(a, z, state_at), carry);
-  const Gate<T, VEC> forget(a.forget_bias), input(0.f);
+  const Gate<T, VEC, true> forget(a.forget_bias);
+  const Gate<T, VEC, false> input(0.f);
   uint32_t cuts = 0, next_cuts = 0;
   if (CUT) next_cuts = load_cuts<STEPS>(a, at.b, t_first, at.lane);
 
@@ -502,7 +546,8 @@ scan_bwd_kernel(const ScanArgs a, const ScanGrads g, const int wide, const int w
 #pragma unroll 4
     for (int z = ch.count * ch.pieces - 1; z >= (at.chunk + 1) * ch.pieces; --z) carry = after<CUT>(ch.run<VEC>(a, z, state_at), carry);
   V next_front = front_of(0);
-  const Gate<T, VEC> forget(a.forget_bias), input(0.f);
+  const Gate<T, VEC, true> forget(a.forget_bias);
+  const Gate<T, VEC, false> input(0.f);
   uint32_t cuts = 0, next_cuts = 0;
   if (CUT) next_cuts = load_cuts<STEPS>(a, at.b, t0_of(0), at.lane);
 
@@ -661,6 +706,13 @@ cudaError_t run_backward(const ScanArgs& a, const ScanGrads& g, float* runs, int
 
 template <typename T, int VEC, int STEPS>
 cudaError_t forward(const ScanArgs& a, void* y, float* last, float* kept, float* runs, int wide, int* launched, cudaStream_t st) {
+  // 128 x 2048 channels with an input gate, us: 1 step 2.9, walked through the ring 6.7; 4 steps 5.0 and 7.3
+  if (a.steps <= kFew) {
+    const long long threads = (long long)(a.channels / VEC) * a.batch;
+    *launched = 1;
+    return launch_pdl(a.input.p != nullptr ? scan_few_kernel<T, VEC, true> : scan_few_kernel<T, VEC, false>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a,
+                      static_cast<T*>(y), last, kept);
+  }
   if (a.reset != nullptr)
     return a.input.p != nullptr ? run_forward<T, VEC, true, true, STEPS>(a, y, last, kept, runs, wide, launched, st) : run_forward<T, VEC, false, true, STEPS>(a, y, last, kept, runs, wide, launched, st);
   return a.input.p != nullptr ? run_forward<T, VEC, true, false, STEPS>(a, y, last, kept, runs, wide, launched, st) : run_forward<T, VEC, false, false, STEPS>(a, y, last, kept, runs, wide, launched, st);

@@ -109,7 +109,7 @@ def _check(s, bias=0.0):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("gate", [False, True])
-@pytest.mark.parametrize("steps", [1, 2, 3, 7, 8, 9, 15, 16, 17, 33, 64, 65, 127, 128, 129, 255, 257, 300, 1025])
+@pytest.mark.parametrize("steps", [1, 2, 3, 4, 5, 7, 8, 9, 15, 16, 17, 33, 64, 65, 127, 128, 129, 255, 257, 300, 1025])
 def test_lengths(dtype, gate, steps):
     _check(_inputs(2, steps, 72, dtype, gate, state=steps % 2 == 1, resets=0.03 if steps % 3 == 0 else None))
 
@@ -128,7 +128,7 @@ def test_shapes_that_are_split_in_their_own_way(dtype, batch, steps, channels):
 
 
 @pytest.mark.parametrize("resets", [0.0, 0.5, 1.0])
-@pytest.mark.parametrize("steps", [5, 200, 1500])
+@pytest.mark.parametrize("steps", [1, 4, 5, 200, 1500])
 def test_resets(resets, steps):
     s = _inputs(2, steps, 70, torch.float32, resets=resets)
     _check(s)
