@@ -9,6 +9,13 @@
 // 512 threads that share it (16 bytes a piece), so that it is read once; thread
 // groups walk along the rows with the weight, and backward the weight's gradient, of their columns in registers too. Rows wider than
 // that are read again for every sum.
+//
+// Measured (B200, replayed back to back; shares of the copy rate): 16384 x 4096 in bf16 with a residual, forward 101 us (0.81), in 8 bits 78
+// (0.92), backward 98 (0.83); 32768 x 1024 in fp32 87, 73, 86 (0.95, 0.92, 0.95); 12289 x 1001 in fp32 without a residual 22 and 35; 8 x 2048
+// 2.4 and 4.7, a launch each. What held it back before was the wait for a row behind every row's sums: with the next row's pieces in
+// registers 151 us backward where rows ahead in shared memory take 98; with the largest size in an exchange of its own 108 us in 8 bits
+// where one exchange for both takes 97, and rows ahead 78. bf16 rows of more than 4096 odd columns keep one block of 512 threads an
+// SM backward (4096 x 8191 143 us, 0.22): the 16 sums and weights of a thread fill its registers.
 #include "rms_norm.h"
 
 #include <cuda_bf16.h>
@@ -491,18 +498,21 @@ __global__ void __launch_bounds__(kThreads) wide_norm_dw_kernel(const NormGrad p
 }
 
 // ------------------------------------------------------------------------------------------------ host
-// How many pieces a thread holds and how many threads share a row: two pieces each where the rows alone fill the SMs (fewer threads to
-// join for each sum), one where a row's latency counts.
+// How many pieces a thread holds and how many threads share a row. One piece where a row's latency counts; where the rows alone fill the SMs
+// two, or four where a warp has the row to itself then (no barrier: 20000 x 300 in fp32 13.3 -> 11.6 us, in 8 bits 15.9 -> 13.4; wider
+// rows lose some: 12288 x 1024 in 8 bits 27.1 -> 28.8). Backward in fp32 four: 4096 x 4096 50.7 -> 47.1 us, 20000 x 300 25.5 -> 17.6;
+// in bf16 their 32 columns a thread do not fit the registers.
 struct Layout { int pieces, group; };       // pieces 0: the row does not fit
-Layout layout_of(long long rows, int width, int vec) {
-  const int all = width % vec == 0 ? width / vec : (width + 2 * vec - 2) / vec, most_pieces = 4;
+Layout layout_of(long long rows, int width, int vec, bool backward) {
+  const int all = width % vec == 0 ? width / vec : (width + 2 * vec - 2) / vec;
   auto group_for = [&](int pieces) {
     int g = 32;
     while (g < 512 && g * pieces < all) g *= 2;
     return g;
   };
-  int pieces = rows >= 4LL * sm_count() ? 2 : 1;
-  while (pieces < most_pieces && group_for(pieces) * pieces < all) pieces *= 2;
+  int pieces = 1;
+  if (rows >= 4LL * sm_count()) pieces = backward ? (vec == 4 ? 4 : 2) : all > 64 && all <= 128 ? 4 : 2;
+  while (pieces < 4 && group_for(pieces) * pieces < all) pieces *= 2;
   const int group = group_for(pieces);
   return group * pieces < all ? Layout{0, 0} : Layout{pieces, group};
 }
@@ -563,7 +573,7 @@ template <typename T, typename W, bool QUANT>
 cudaError_t forward(const NormRows& p, void* y, void* codes, long long codes_ld, float* scales, cudaStream_t st) {
   if (p.rows <= 0) return cudaSuccess;
   const Kind kind = kind_of(p, y);
-  const Layout l = layout_of(p.rows, p.width, 16 / sizeof(T));
+  const Layout l = layout_of(p.rows, p.width, 16 / sizeof(T), false);
   if (l.pieces != 0) {
     if (kind == kAligned) return forward_rows<T, W, QUANT, kAligned>(p, l, y, codes, codes_ld, scales, st);
     if (kind == kShifted) return forward_rows<T, W, QUANT, kShifted>(p, l, y, codes, codes_ld, scales, st);
@@ -582,7 +592,7 @@ cudaError_t forward_of(const NormRows& p, void* y, void* codes, long long codes_
 constexpr int kWideParts = 64;
 constexpr int kThreadsBack = 512;            // on an SM, twice as many where a thread has 8 columns at most
 
-Layout layout_back(const NormGrad& p) { return layout_of(p.rows, p.width, p.bf16 ? 8 : 4); }
+Layout layout_back(const NormGrad& p) { return layout_of(p.rows, p.width, p.bf16 ? 8 : 4, true); }
 long long blocks_back(const NormGrad& p, const Layout& l) {
   const int block = block_of(l.group), beside = block / l.group, vec = p.bf16 ? 8 : 4;
   const long long most = (long long)sm_count() * (kThreadsBack / block) * (l.pieces * vec <= 8 ? 2 : 1);
