@@ -8,9 +8,8 @@
 // mean. The random 16 bits are a hash of (seed, step, place), so a step can be repeated. A size that is not zero never becomes the
 // value zero: a lost root would divide by eps alone.
 //
-// Measured (B200, fp32 parameters and gradients): 143 M parameters in 34 tensors, 8 bits 464 us (0.75 of the copy rate: 80 instructions a
-// parameter, a third of them the hash and the two roundings, of which the memory would allow 88 with every issue slot taken), 32 bits
-// 715 (0.85); 80 tensors of 4001 9.1 and 6.7. Steps that gave it: eight neighbours a lane 1278 -> 788 us, one hash for two of them and
+// Measured (B200, fp32 parameters and gradients): 143 M parameters in 34 tensors, 8 bits 464 us (0.75 of the copy rate: 79 instructions a
+// parameter, of which the memory would allow 88 with every issue slot taken), 32 bits 720 (0.85); 80 tensors of 4001 9.1 and 6.9. Steps that gave it: eight neighbours a lane 1278 -> 788 us, one hash for two of them and
 // the rounding on exponents that coincide 634, 64 registers and the integer maximum of a warp 464.
 #include "adamw_list.h"
 

@@ -10,9 +10,9 @@
 //           the contraction is split over a cluster where the tiles leave SMs idle, and summed through distributed shared memory in a
 //           fixed order: decoding steps, bound by reading the weight
 //
-// Measured (B200, replayed back to back, operands in the L2 where they fit): 8192 x 4096 x 4096 97 us, 2846 TFLOP/s, 0.85 of twice the bf16
-// burst rate; 8192 x 512 x 4096 25 us, bound by draining 74 tiles of 128 KB at a time (44 us with a row a lane, whose scales were read in
-// the drain instead of ahead of it); 1024 x 4096 x 4096 16; 8 x 2048 x 8192 5.2 us, of which a launch and a first tile are 3.
+// Measured (B200, replayed back to back, operands in the L2 where they fit; rows x contraction x columns): 8192 x 4096 x 4096 97 us, 2846 TFLOP/s,
+// 0.85 of twice the bf16 burst rate; 1024 x 4096 x 4096 16; 8192 x 512 x 4096 25 us, of which memory and tensor cores need 11 and 10 each
+// (44 us when a lane drained a row of its own instead of fragments); 8 x 2048 x 8192 5.2 us, 3 of them by the weight's bytes.
 #include "gemm_8bit.h"
 
 #include <cuda.h>

@@ -19,10 +19,10 @@
 //
 // Measured (B200, replayed back to back, bf16; share of the copy rate by the bytes that have to move): 32 x 2048 x 1024 forward 72 us (0.85),
 // backward 136 (0.75); 1 x 65536 x 1024 127 (0.48; its inputs are read twice) and 182 (0.56); 128 x 20 x 2048 with an input gate 12.8
-// (0.50) and 18.7 (0.60); in fp32 1 x 32768 x 1024 106 and 152. What bounds them is issuing instructions, 19 a value forward and 39
+// (0.50) and 18.7 (0.60); in fp32 1 x 32768 x 1024 108 and 152. What bounds them is issuing instructions, 19 a value forward and 39
 // backward, of which the memory would allow 33 and 55 with every issue slot taken: so values go in pairs, gates stay in registers
 // (8 or 16 steps of a warp: what 128 registers hold at 16 warps an SM), and inputs are read again from shared memory instead of
-// being kept (32 x 2048 x 1024 backward 156 -> 132).
+// being kept (32 x 2048 x 1024 backward 156 -> 136).
 //
 // The states are not stored: the forward pass keeps them in fp32 in front of every tile of the backward pass, which walks the other way with
 // the same joining of dh and computes those in between again. States, gates and sums are fp32.
@@ -706,7 +706,7 @@ cudaError_t run_backward(const ScanArgs& a, const ScanGrads& g, float* runs, int
 
 template <typename T, int VEC, int STEPS>
 cudaError_t forward(const ScanArgs& a, void* y, float* last, float* kept, float* runs, int wide, int* launched, cudaStream_t st) {
-  // 128 x 2048 channels with an input gate, us: 1 step 2.9, walked through the ring 6.7; 4 steps 5.0 and 7.3
+  // 128 x 2048 channels with an input gate, us: 1 step 2.6, walked through the ring 6.7; 4 steps 4.7 and 7.3
   if (a.steps <= kFew) {
     const long long threads = (long long)(a.channels / VEC) * a.batch;
     *launched = 1;

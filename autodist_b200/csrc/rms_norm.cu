@@ -6,16 +6,15 @@
 //   dx = ds + rstd * (g - n * mean(g n)),  dw = sum over rows of dy * n,  with g = dy * w, n = s * rstd
 //
 // Sums are fp32. Memory-bound: a few operations for each element that is read and written once. A row stays in the registers of the 32 to
-// 512 threads that share it (16 bytes a piece), so that it is read once; thread
-// groups walk along the rows with the weight, and backward the weight's gradient, of their columns in registers too. Rows wider than
-// that are read again for every sum.
+// 512 threads that share it (16 bytes a piece), so that it is read once; thread groups walk along the rows with the weight, and backward
+// the weight's gradient, of their columns in registers too. Rows wider than that are read again for every sum.
 //
 // Measured (B200, replayed back to back; shares of the copy rate): 16384 x 4096 in bf16 with a residual, forward 101 us (0.81), in 8 bits 78
-// (0.92), backward 98 (0.83); 32768 x 1024 in fp32 87, 73, 86 (0.95, 0.92, 0.95); 12289 x 1001 in fp32 without a residual 22 and 35; 8 x 2048
+// (0.92), backward 98 (0.83); 32768 x 1024 in fp32 86, 74, 86 (0.95, 0.90, 0.95); 12289 x 1001 in fp32 without a residual 22 and 35; 8 x 2048
 // 2.4 and 4.7, a launch each. What held it back before was the wait for a row behind every row's sums: with the next row's pieces in
 // registers 151 us backward where rows ahead in shared memory take 98; with the largest size in an exchange of its own 108 us in 8 bits
-// where one exchange for both takes 97, and rows ahead 78. bf16 rows of more than 4096 odd columns keep one block of 512 threads an
-// SM backward (4096 x 8191 143 us, 0.22): the 16 sums and weights of a thread fill its registers.
+// where one exchange for both takes 97, and rows ahead 78. What it has not solved are wide bf16 rows of an odd width: 4096 x 8191 takes 64
+// us forward and 143 backward (0.32 and 0.21), with two pieces a thread at 122 registers and so one block of 512 threads an SM backward.
 #include "rms_norm.h"
 
 #include <cuda_bf16.h>
