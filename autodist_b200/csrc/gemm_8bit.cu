@@ -12,7 +12,8 @@
 //
 // Measured (B200, replayed back to back, operands in the L2 where they fit; rows x contraction x columns): 8192 x 4096 x 4096 97 us, 2846 TFLOP/s,
 // 0.85 of twice the bf16 burst rate; 1024 x 4096 x 4096 16; 8192 x 512 x 4096 25 us, of which memory and tensor cores need 11 and 10 each
-// (44 us when a lane drained a row of its own instead of fragments); 8 x 2048 x 8192 5.2 us, 3 of them by the weight's bytes.
+// (44 us when a lane drained a row of its own instead of fragments); 8 x 2048 x 8192 5.2 us (the weight's bytes from
+// memory alone would take 2.6).
 #include "gemm_8bit.h"
 
 #include <cuda.h>
