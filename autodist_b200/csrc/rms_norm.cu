@@ -13,8 +13,9 @@
 // (0.92), backward 98 (0.83); 32768 x 1024 in fp32 86, 74, 86 (0.95, 0.90, 0.95); 12289 x 1001 in fp32 without a residual 22 and 35; 8 x 2048
 // 2.4 and 4.7, a launch each. What held it back before was the wait for a row behind every row's sums: with the next row's pieces in
 // registers 151 us backward where rows ahead in shared memory take 98; with the largest size in an exchange of its own 108 us in 8 bits
-// where one exchange for both takes 97, and rows ahead 78. What it has not solved are wide bf16 rows of an odd width: 4096 x 8191 takes 64
-// us forward and 143 backward (0.32 and 0.21), with two pieces a thread at 122 registers and so one block of 512 threads an SM backward.
+// where one exchange for both takes 97, and rows ahead 78. What it has not solved are the widest
+// odd rows in bf16: 4096 x 8191 takes 64 us forward and 121 backward where 8185 columns take 34 and 69, since its 1025 pieces need four a
+// thread.
 #include "rms_norm.h"
 
 #include <cuda_bf16.h>
@@ -500,14 +501,14 @@ __global__ void __launch_bounds__(kThreads) wide_norm_dw_kernel(const NormGrad p
 // How many pieces a thread holds and how many threads share a row. One piece where a row's latency counts; where the rows alone fill the SMs
 // two, or four where a warp has the row to itself then (no barrier: 20000 x 300 in fp32 13.3 -> 11.6 us, in 8 bits 15.9 -> 13.4; wider
 // rows lose some: 12288 x 1024 in 8 bits 27.1 -> 28.8). Backward in fp32 four: 4096 x 4096 50.7 -> 47.1 us, 20000 x 300 25.5 -> 17.6;
-// in bf16 their 32 columns a thread do not fit the registers.
+// in bf16 their 32 columns a thread do not fit the registers. Groups are whole warps rather than powers of two: 4096 rows in bf16 of 4095
+// columns 31.9 / 69.6 -> 26.5 / 55.0 us, of 2047 16.9 / 35.6 -> 16.2 / 26.0, 3000 in fp32 22.5 / 29.2 -> 19.6 / 27.8; 6001 forward 32.0 -> 33.9.
 struct Layout { int pieces, group; };       // pieces 0: the row does not fit
 Layout layout_of(long long rows, int width, int vec, bool backward) {
   const int all = width % vec == 0 ? width / vec : (width + 2 * vec - 2) / vec;
   auto group_for = [&](int pieces) {
-    int g = 32;
-    while (g < 512 && g * pieces < all) g *= 2;
-    return g;
+    const int warps = (all + 32 * pieces - 1) / (32 * pieces);
+    return 32 * (warps < 16 ? warps : 16);
   };
   int pieces = 1;
   if (rows >= 4LL * sm_count()) pieces = backward ? (vec == 4 ? 4 : 2) : all > 64 && all <= 128 ? 4 : 2;
@@ -515,7 +516,7 @@ Layout layout_of(long long rows, int width, int vec, bool backward) {
   const int group = group_for(pieces);
   return group * pieces < all ? Layout{0, 0} : Layout{pieces, group};
 }
-int block_of(int group) { return group < 256 ? 256 : group; }
+int block_of(int group) { return group < 256 ? 256 / group * group : group; }
 
 bool aligned(const void* p, long long ld, int bytes) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * bytes % 16 == 0; }
 Kind kind_of(const NormRows& p, const void* y) {

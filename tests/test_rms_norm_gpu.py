@@ -78,6 +78,30 @@ def test_gradient_of_a_shared_weight_over_many_rows(rows, width):
     assert torch.equal(first, torch.autograd.grad(F.rms_norm(x, w, eps=EPS), w, dy)[0])       # the order of the sums is fixed
 
 
+@pytest.mark.parametrize("width", [159, 161, 519, 520, 1025, 1301, 2047, 2560, 4095, 5001, 8185, 8191])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_many_rows_with_groups_of_any_number_of_warps(width, dtype):
+    from autodist_b200.ops import functional as F
+    x, w, res, dy, ds = _inputs(1203, width, dtype)
+    s, n, rstd, y = _reference(x, w, res)
+    codes, scales, total = F.rms_norm_8bit(x, w, res, EPS)
+    assert torch.equal(total, s)
+    most = y.abs().amax(1, keepdim=True)
+    step = most / 448
+    _near(scales.reshape(-1, 1), step, 2 * SUMS * step)
+    _near(codes.double() * scales.double().reshape(-1, 1), y, (2.0 ** -4 + 4 * SUMS) * y.abs() + step * 2.0 ** -10)
+    leaves = [t.requires_grad_(True) for t in (x, w, res)]
+    out = F.rms_norm(x, w, res, EPS)
+    _near(out[0], y, (ROUND[dtype] + SUMS) * y.abs())
+    grads = torch.autograd.grad(out, leaves, (dy, ds))
+    g = dy.double() * w.double()
+    dx = rstd * (g - n * (g * n).mean(-1, keepdim=True)) + ds.double()
+    sizes = rstd * (g.abs() + n.abs() * (g * n).abs().mean(-1, keepdim=True)) + ds.double().abs()
+    _near(grads[0], dx, ROUND[dtype] * dx.abs() + 2 * SUMS * sizes)
+    dw = (dy.double() * n).sum(0)
+    _near(grads[1], dw, ROUND[torch.float32] * dw.abs() + 2 * SUMS * (dy.double() * n).abs().sum(0))
+
+
 @pytest.mark.parametrize("width", WIDTHS)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_output_in_8_bits(width, dtype):
