@@ -14,7 +14,7 @@
 // 2.4 and 4.7, a launch each. What held it back before was the wait for a row behind every row's sums: with the next row's pieces in
 // registers 151 us backward where rows ahead in shared memory take 98; with the largest size in an exchange of its own 108 us in 8 bits
 // where one exchange for both takes 97, and rows ahead 78. What it has not solved are the widest
-// odd rows in bf16: 4096 x 8191 takes 64 us forward and 121 backward where 8185 columns take 34 and 69, since its 1025 pieces need four a
+// odd rows in bf16: 4096 x 8191 takes 64 us forward and 119 backward where 8185 columns take 34 and 69, since its 1025 pieces need four a
 // thread.
 #include "rms_norm.h"
 
@@ -99,22 +99,34 @@ template <int VEC, bool SHIFT, typename W> __device__ __forceinline__ void load_
     for (int i = 0; i < VEC; i += 4) Piece<float, 4>::unpack(Piece<float, 4>::load(w + i), v + i);
   }
 }
+// Codes of a row's columns c ... Shifted ones are stored in twos, from the second on where the first lies on an odd address, and only those at
+// a row's ends are looked at one by one: 4096 rows of 4095 columns in bf16 34.7 -> 29.0 us, of 8185 68.8 -> 54.6; in fp32 no change (12289 x
+// 1001 25). To put them together into words with the next lane's takes longer, 72 and 78 us, since a warp's ends are then left over.
 template <int VEC, bool SHIFT> __device__ __forceinline__ void store_codes(uint8_t* p, int c, int width, const float* v) {
+  uint32_t w[VEC / 4];
+#pragma unroll
+  for (int i = 0; i < VEC / 4; ++i) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i], v[4 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i + 2], v[4 * i + 3]), __NV_SATFINITE, __NV_E4M3);
+    w[i] = lo | hi << 16;
+  }
+  auto code = [&](int j) { return w[j / 4] >> 8 * (j % 4); };
   p += c;
-  if constexpr (SHIFT) {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j)
-      if (c + j >= 0 && c + j < width) p[j] = __nv_cvt_float_to_fp8(v[j], __NV_SATFINITE, __NV_E4M3);
-  } else {
-    uint32_t w[VEC / 4];
-#pragma unroll
-    for (int i = 0; i < VEC / 4; ++i) {
-      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i], v[4 * i + 1]), __NV_SATFINITE, __NV_E4M3);
-      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i + 2], v[4 * i + 3]), __NV_SATFINITE, __NV_E4M3);
-      w[i] = lo | hi << 16;
-    }
+  if constexpr (!SHIFT) {
     if constexpr (VEC == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
     else *reinterpret_cast<uint32_t*>(p) = w[0];
+  } else if (c < 0 || c + VEC > width) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j)
+      if (c + j >= 0 && c + j < width) p[j] = (uint8_t)code(j);
+  } else if (reinterpret_cast<uintptr_t>(p) & 1) {
+    p[0] = (uint8_t)code(0);
+#pragma unroll
+    for (int j = 1; j < VEC - 1; j += 2) *reinterpret_cast<uint16_t*>(p + j) = (uint16_t)(j % 4 == 3 ? __funnelshift_r(w[j / 4], w[(j + 1) / 4], 24) : code(j));
+    p[VEC - 1] = (uint8_t)code(VEC - 1);
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; j += 2) *reinterpret_cast<uint16_t*>(p + j) = (uint16_t)code(j);
   }
 }
 
