@@ -317,3 +317,22 @@ def test_refusals():
         E.gated_scan_fwd(x.cpu(), x, None, None, None, 0.0, False)
     with pytest.raises(RuntimeError, match="states needed"):
         E.gated_scan_bwd(x, None, x, x, None, None, None, torch.zeros(3, device="cuda"), 0.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("gate", [False, True])
+@pytest.mark.parametrize("batch,steps,channels", [(2, 1, 8), (3, 37, 33), (1, 3001, 64)])
+def test_training_calls_leave_their_inputs_alone(batch, steps, channels, gate, dtype):
+    from autodist_b200.ops import functional as F
+    g = torch.Generator(device="cuda").manual_seed(steps)
+    x, forget, i, dy = (torch.randn(batch, steps, channels, generator=g, device="cuda").to(dtype) for _ in range(4))
+    state, dlast = (torch.randn(batch, channels, generator=g, device="cuda") for _ in range(2))
+    inputs = [x, forget, state, dy, dlast] + ([i] if gate else [])
+    before = [t.clone() for t in inputs]
+    leaves = [t.requires_grad_(True) for t in ([x, forget, i, state] if gate else [x, forget, state])]
+    results = []
+    for _ in range(3):
+        out = F.gated_recurrence(x, forget, i if gate else None, state=state)
+        results.append(list(out) + list(torch.autograd.grad(out, leaves, (dy, dlast))))
+    assert all(torch.equal(a, b.detach()) for a, b in zip(before, inputs))
+    assert all(torch.equal(a, b) for later in results[1:] for a, b in zip(results[0], later))
